@@ -10,7 +10,9 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import math
 from ctypes import c_float, c_int, c_void_p
+from typing import NamedTuple
 
 import torch
 
@@ -119,6 +121,9 @@ def _signatures(lib) -> None:
         "pl_parallel_step": [p, p, p, p, p, p, p, p, f, p, p, i, p, i, i, f, p, p, p, p, i, i, ctypes.c_longlong, p],
         "pl_gemm_tiled_grouped": [p, p, p, p, p, ctypes.c_longlong, i, i, i, i, i, i, i, f, i, i, i, p, i, i, p],
         "pl_sandwich_step": [p, p, p, p, f, p, p, f, p, i, p, i, i, i, p],
+        "pl_step_tables": [p, p, i, p, i, i, p, i, i, p, p, p, p, p, p],
+        "pl_qk_norm_rope_kv_write_8bit": [p, p, i, p, p, i, f, p, p, i, i, i, p, p, i, i, p, p, p, p, i, i, i, i, i, p],
+        "pl_paged_attention_8bit": [p, i, p, p, p, p, i, i, i, p, i, i, i, p, p, p, p, i, i, i, f, i, i, i, p, p, i, p],
         "pl_bigram_add": [p, p, p, p, p, p, p, p, p, p, p, i, ctypes.c_longlong, ctypes.c_longlong, ctypes.c_longlong, i, i, p],
     }
     for name, argtypes in table.items():
@@ -2912,3 +2917,173 @@ def bigram_add_(x: torch.Tensor, batch, table: torch.Tensor, last: torch.Tensor,
                                    batch.state_slots.data_ptr(), last.data_ptr(), table.data_ptr(), _code(table, "table of pairs of tokens"),
                                    int(mul_prev), int(mul_cur), table.shape[0] - 1, n, W, _stream()))
     return x
+
+
+# ---------------------------------------------------------------------------
+# A paged cache held in 8 bits: pages of e4m3 values [pages * page size, key heads * head size] for keys and for values, and for each of the two a power of
+# two a page and key head [pages, key heads] that the values are multiplied by.
+
+E4M3, E8M0 = torch.float8_e4m3fn, torch.float8_e8m0fnu
+STEP_TABLES_MAX_SEQS = 8192
+
+
+class StepTables(NamedTuple):
+    """Where a step's tokens stand and go, made on the GPU (all int32): see ``step_tables``."""
+    positions: torch.Tensor     # [rows]
+    seq_of: torch.Tensor        # [rows]
+    slots: torch.Tensor         # [rows]
+    q_start: torch.Tensor       # [requests]
+    pages: torch.Tensor         # [1]
+
+
+def _here(t: torch.Tensor, what: str) -> None:
+    """Launches go to the current device's stream: a tensor of another device would be read from there."""
+    if t.device.index != torch.cuda.current_device():
+        raise TensorError(f"{what} is on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
+
+
+def step_tables(q_len: torch.Tensor, ctx_len: torch.Tensor, block_table: torch.Tensor, block_size: int, free_pages: torch.Tensor | None, rows: int) -> StepTables:
+    """Block tables and slots of a step from its requests' lengths, without a word from the host.  Request s brings ``q_len[s]`` tokens and has ``ctx_len[s]`` behind the
+    step; the rows of the requests follow each other from row 0.  ``positions``, ``seq_of`` and ``slots`` (page * ``block_size`` + place in the page) of every row, ``q_start`` of every request.
+
+    With ``free_pages`` (page numbers, in the order in which they are handed out) the pages that a request needs beyond those of its first ctx_len - q_len tokens are taken from there,
+    request after request, and written into its row of ``block_table``; the entries behind a request's pages become -1.  ``pages`` is how many they need together: where the list or a row of the table
+    is shorter, entries and slots past its end are -1 (the slots of a table that is too narrow) and ``pages`` counts what the table's rows have room for, so more than ``len(free_pages)`` says that pages are missing.
+    With None the table is read as it stands and written by nobody, and ``pages`` is 0.
+
+    Rows behind the last request's, up to ``rows``, and those of a request whose context is shorter than what it brings (the padding of a step) have position and slot -1;
+    ``seq_of`` of rows behind the last is the last request."""
+    _need(q_len, "tokens of each request", None, torch.int32)
+    S = q_len.numel()
+    _need(ctx_len, "context length of each request", (S,), torch.int32)
+    _need(block_table, "block table", None, torch.int32)
+    _here(block_table, "block table")
+    if q_len.dim() != 1 or not 1 <= S <= STEP_TABLES_MAX_SEQS:
+        raise TensorError(f"tokens of each request have shape {tuple(q_len.shape)}, expected [1 to {STEP_TABLES_MAX_SEQS}]")
+    if block_table.dim() != 2 or block_table.shape[0] != S or block_table.shape[1] < 1:
+        raise TensorError(f"block table has shape {tuple(block_table.shape)}, expected [{S}, pages]")
+    if free_pages is not None:
+        _need(free_pages, "free pages", (free_pages.numel(),), torch.int32)
+    if rows < 0 or block_size < 1:
+        raise TensorError(f"{rows} rows of pages of {block_size} tokens")
+    made = StepTables(*torch.empty(3 * rows + S + 1, dtype=torch.int32, device=q_len.device).split([rows, rows, rows, S, 1]))
+    # (an empty list of free pages is a list: its address may be nothing, and any other stands for it)
+    free = 0 if free_pages is None else (free_pages.data_ptr() or block_table.data_ptr())
+    _check(library().pl_step_tables(q_len.data_ptr(), ctx_len.data_ptr(), S, block_table.data_ptr(), block_table.shape[1], block_size, free,
+                                    0 if free_pages is None else free_pages.numel(), rows, made.q_start.data_ptr(), made.positions.data_ptr(), made.seq_of.data_ptr(),
+                                    made.slots.data_ptr(), made.pages.data_ptr(), _stream()))
+    return made
+
+
+def _pages_8bit(k_pool, v_pool, k_scale, v_scale, block_size: int, nkv: int, d: int) -> int:
+    """The rows of the pools, once they are what the kernels take."""
+    if not 16 <= d <= 256 or d % 16:
+        raise TensorError(f"head size {d}: the 8-bit cache takes multiples of 16 up to 256")
+    _need(k_pool, "key pool", None, E4M3)
+    rows = k_pool.shape[0]
+    if block_size < 1 or nkv < 1 or k_pool.dim() != 2 or k_pool.shape[1] != nkv * d or rows % block_size or rows == 0:
+        raise TensorError(f"key pool has shape {tuple(k_pool.shape)}, expected [pages*{block_size}, {nkv * d}]")
+    if rows >= 2 ** 31:
+        raise TensorError("a pool of 2^31 slots or more is not addressed by these kernels")
+    _need(v_pool, "value pool", k_pool.shape, E4M3)
+    pages = (rows // block_size, nkv)
+    _need(k_scale, "powers of the keys", pages, E8M0)
+    _need(v_scale, "powers of the values", pages, E8M0)
+    if not in_pieces(k_pool, v_pool):
+        raise TensorError("the pools of an 8-bit cache begin at whole 16 bytes")
+    _here(k_pool, "key pool")
+    return rows
+
+
+def qk_norm_rope_kv_write_8bit(qkv: torch.Tensor, q: torch.Tensor | None, q_gain, k_gain, eps: float, cos, sin, rot: int, positions: torch.Tensor, slots: torch.Tensor,
+                               block_size: int, k_pool: torch.Tensor, v_pool: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor, nq: int, nkv: int, d: int,
+                               neighbours: bool = False, write_kv: bool = True) -> None:
+    """What ``qk_norm_rope_kv_write`` does, into a cache held in 8 bits: per-head norm and rotation of q and k at each token's position, q into ``q`` [rows, nq * d] (None: in place inside
+    ``qkv``), k and v into the slots of their pages as e4m3, rounded to nearest.  A page's power of two (a key head's, keys and values apart) becomes the least whose 448-fold holds
+    the largest finite value that the page holds of this request and is given; where it grows, what the page holds is rounded again in the new unit.  A page whose first slot is written begins anew.
+    What is not finite is kept as NaN.
+
+    The rows that go into one page follow each other with slots that follow each other, as those of a request's tokens do, and no page is named twice; a slot below 0 (or past the
+    pool) is written nowhere, and the queries of a row with a position below 0 are left as they were.  ``write_kv=False``: the queries alone."""
+    n = qkv.shape[0]
+    code = _code(qkv, "fused q/k/v projection")
+    _need(qkv, "fused q/k/v projection", (n, (nq + 2 * nkv) * d))
+    rows = _pages_8bit(k_pool, v_pool, k_scale, v_scale, block_size, nkv, d)
+    _need(positions, "positions", (n,), torch.int32)
+    _need(slots, "slots", (n,), torch.int32)
+    if q is None:
+        q, stride = qkv, qkv.shape[1]
+    else:
+        _need(q, "queries", (n, nq * d), qkv.dtype)
+        stride = nq * d
+    gain_code = F32
+    if (q_gain is None) != (k_gain is None):
+        raise TensorError("queries and keys are normed both or neither")
+    if q_gain is not None:
+        _need(q_gain, "query norm gain", (d,))
+        _need(k_gain, "key norm gain", (d,), q_gain.dtype)
+        gain_code = _code(q_gain, "query norm gain")
+    if rot:
+        _need(cos, "cosine table", None, torch.float32)
+        if rot % 2 or not 0 < rot <= d or cos.dim() != 2 or cos.shape[1] != rot // 2 or cos.shape[0] < 1:
+            raise TensorError(f"rotary tables have shape {tuple(cos.shape)}, expected [positions, {rot // 2}] for a rotation over {rot} values of a head of {d}")
+        _need(sin, "sine table", cos.shape, torch.float32)
+    if not in_pieces(qkv, q, q_gain, k_gain):
+        raise TensorError("rows and gains for an 8-bit cache begin at whole 16 bytes")
+    _check(library().pl_qk_norm_rope_kv_write_8bit(
+        qkv.data_ptr(), q.data_ptr(), stride, _ptr(q_gain), _ptr(k_gain), gain_code, eps, cos.data_ptr() if rot else 0, sin.data_ptr() if rot else 0, rot,
+        cos.shape[0] if rot else 0, 1 if neighbours else 0, positions.data_ptr(), slots.data_ptr() if write_kv else 0, block_size, rows, k_pool.data_ptr(), v_pool.data_ptr(),
+        k_scale.data_ptr(), v_scale.data_ptr(), n, nq, nkv, d, code, _stream()))
+
+
+def shares_8bit(n: int, requests: int, max_ctx: int, nq: int, nkv: int, window: int = 0) -> tuple:
+    """(keys a share, shares) of the 8-bit attention's few-row kernel."""
+    reach = max_ctx if window <= 0 else min(max_ctx, window + 32)
+    chunk = 512
+    shares = (max_ctx + chunk - 1) // chunk
+    return chunk, min(shares, reach // chunk + 2) if window > 0 else shares
+
+
+def paged_attention_8bit(q: torch.Tensor, q_row_stride: int, out: torch.Tensor, q_start: torch.Tensor, q_len: torch.Tensor, ctx_len: torch.Tensor, max_q_len: int,
+                         max_ctx: int, block_table: torch.Tensor, block_size: int, k_pool: torch.Tensor, v_pool: torch.Tensor, k_scale: torch.Tensor,
+                         v_scale: torch.Tensor, nq: int, nkv: int, d: int, scale: float, window: int = 0, min_q_len: int = 1) -> torch.Tensor:
+    """Attention over a cache held in 8 bits, for any mixture of single tokens, drafts and portions of prompts, in bfloat16 and in 32 bits.  Request s brings the rows q_start[s] ..
+    q_start[s]+q_len[s]-1 at the positions ctx_len[s]-q_len[s] .. ctx_len[s]-1, whose keys and values are in the cache already; a row sees the keys up to its own, under ``window`` > 0 the last so
+    many of them, under ``window`` < 0 those of its own block of -window positions.  ``q`` rows begin with the rotated queries, ``q_row_stride`` apart.  Rows of no request, and of requests whose context is shorter than what they bring, are left
+    as they were in ``out``.
+
+    ``max_q_len``, ``min_q_len`` and ``max_ctx`` bound what the requests bring and their contexts (the launches are sized and chosen by them): rows whose keys reach past ``max_ctx`` come out as NaN, and
+    rows past ``max_q_len`` of a request may be left out.  The caller answers for the pages of all keys that are seen; keys that no row of a request sees may hold anything."""
+    n = q.shape[0]
+    code = _code(q, "query buffer")
+    _need(q, "query buffer")
+    if q.dim() != 2 or n < 1 or q.shape[1] != q_row_stride or q_row_stride < nq * d:
+        raise TensorError(f"query buffer has shape {tuple(q.shape)} for row stride {q_row_stride}")
+    if nkv < 1 or nq < 1 or nq % nkv:
+        raise TensorError(f"{nq} query heads over {nkv} key heads, which do not group evenly")
+    rows = _pages_8bit(k_pool, v_pool, k_scale, v_scale, block_size, nkv, d)
+    _need(out, "attention output", (n, nq * d), q.dtype)
+    _need(block_table, "block table", None, torch.int32)
+    S = block_table.shape[0]
+    if block_table.dim() != 2 or S < 1 or block_table.shape[1] < 1:
+        raise TensorError(f"block table has shape {tuple(block_table.shape)}, expected [requests, pages]")
+    _need(q_start, "first row of each request", (S,), torch.int32)
+    _need(q_len, "tokens of each request", (S,), torch.int32)
+    _need(ctx_len, "context length of each request", (S,), torch.int32)
+    if not 1 <= max_q_len <= n or not 0 <= min_q_len <= max_q_len or max_ctx < 1:
+        raise TensorError(f"requests are said to bring {min_q_len} to {max_q_len} of the step's {n} tokens, contexts to be {max_ctx} at most")
+    if not 0 < scale < math.inf:
+        raise TensorError(f"scores scaled by {scale}, which has to be finite and above zero")
+    if q_row_stride % 8 or not in_pieces(q, out):
+        raise TensorError("query rows and outputs for an 8-bit cache begin at whole 16 bytes")
+    chunk, chunks = shares_8bit(n, S, int(max_ctx), nq, nkv, int(window or 0))
+    acc = ml = 0
+    if chunks > 1:
+        room = torch.empty(n * nq * chunks * (d + 2), dtype=torch.float32, device=q.device)
+        acc = room.data_ptr()
+        ml = acc + 4 * n * nq * chunks * d
+    _check(library().pl_paged_attention_8bit(
+        q.data_ptr(), q_row_stride, out.data_ptr(), q_start.data_ptr(), q_len.data_ptr(), ctx_len.data_ptr(), S, n, max_q_len, block_table.data_ptr(),
+        block_table.shape[1], block_size, rows, k_pool.data_ptr(), v_pool.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), nq, nkv, d, scale, int(window or 0),
+        chunk, chunks, acc, ml, code, _stream()))
+    return out
