@@ -26,8 +26,7 @@ typedef uint32_t a8_u32x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((__vector_size__(4 * sizeof(__bf16)))) __bf16 a8_bf16x4;
 typedef __attribute__((address_space(3))) a8_bf16x4 a8_lds_bf16x4;
 
-#define A8_ROWS 32       // rows a wave
-#define A8_KEYS 32       // keys a tile
+#define A8_KEYS 32       // keys a wave's tile where every wave has keys of its own
 #define A8_WAVES 4
 
 union a8_frag {
@@ -69,10 +68,6 @@ __device__ __forceinline__ a8_u32x2 a8_read_transposed(const uint16_t* at) {
     return __builtin_bit_cast(a8_u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4bf16((a8_lds_bf16x4*)(at)));
 }
 
-// Elements that a row of values in LDS is padded by: a row then begins 16 banks (of 64) further than the one before, so the four rows of 64 bytes
-// that 32 lanes read transposed fall on every bank once.
-__host__ __device__ constexpr int a8_pad(int dt) { return dt % 2 == 0 ? 32 : 0; }
-
 template <int PIECES>
 struct A8Type;
 template <>
@@ -103,14 +98,24 @@ __device__ __forceinline__ void a8_split(const float (&x)[8], a8_frag (&to)[PIEC
     }
 }
 
-// Which request and which of its blocks of rows is number `slot`, counted over the requests one after the other; by a whole wave.
-__device__ __forceinline__ bool a8_find(const A8Args& a, int slot, int group, int rows, int& seq, int& block) {
+// Whether request s brings rows.  (One whose context is shorter than what it brings holds the rows of a padded step.)
+__device__ __forceinline__ bool a8_brings(const A8Args& a, int s) {
+    return a.q_len[s] > 0 && a.ctx_len[s] >= a.q_len[s] && a.q_start[s] >= 0 && a.q_start[s] <= a.n - a.q_len[s];
+}
+
+// Rows that a request and key head bring are at most this many for the kernel of few rows (so many of its blocks of 16 as the registers hold, see A8Few), more for the kernel of many.
+template <int PIECES, int DQ>
+struct A8Few {
+    static constexpr int BLOCKS = PIECES == 1 ? (DQ <= 2 ? 4 : 2) : (DQ == 1 ? 4 : DQ == 2 ? 2 : 1);
+};
+
+// Which request and which of its blocks of rows is number `slot`, counted over the requests of more than `few` rows one after the other; by a whole wave.
+__device__ __forceinline__ bool a8_find(const A8Args& a, int slot, int group, int rows, int few, int& seq, int& block) {
     const int lane = threadIdx.x % PL_WAVE;
     for (int base = 0; base < a.S; base += PL_WAVE) {
         const int s = base + lane;
         int blocks = 0;
-        // (a request whose context is shorter than what it brings holds the rows of a padded step)
-        if (s < a.S && a.q_len[s] > 0 && a.ctx_len[s] >= a.q_len[s] && a.q_start[s] >= 0 && a.q_start[s] <= a.n - a.q_len[s]) blocks = pl_ceil_div(a.q_len[s] * group, rows);
+        if (s < a.S && a8_brings(a, s) && a.q_len[s] * group > few) blocks = pl_ceil_div(a.q_len[s] * group, rows);
         int end = blocks;
 #pragma unroll
         for (int off = 1; off < PL_WAVE; off <<= 1) {
@@ -120,8 +125,9 @@ __device__ __forceinline__ bool a8_find(const A8Args& a, int slot, int group, in
         const uint64_t past = __ballot(end > slot);
         if (past != 0) {
             const int first = __ffsll(static_cast<unsigned long long>(past)) - 1;
-            seq = base + first;
-            block = slot - (__shfl(end, first, PL_WAVE) - __shfl(blocks, first, PL_WAVE));
+            seq = __builtin_amdgcn_readfirstlane(base + first);
+            // (the last rows, which see the most keys, first)
+            block = __builtin_amdgcn_readfirstlane(__shfl(end, first, PL_WAVE) - 1 - slot);
             return true;
         }
         slot -= __shfl(end, PL_WAVE - 1, PL_WAVE);
@@ -132,70 +138,349 @@ __device__ __forceinline__ bool a8_find(const A8Args& a, int slot, int group, in
 // The keys [lo, hi) that a block of rows sees, cut into shares of `chunk` that begin at whole chunks: how many there are.
 __device__ __forceinline__ int a8_shares(int lo, int hi, int chunk) { return hi > lo ? (hi - 1) / chunk - lo / chunk + 1 : 0; }
 
+// Where key `key` of request `seq` is in the pools, and its page.  (What the table does not say is read from page 0.)
+__device__ __forceinline__ int a8_slot(const A8Args& a, int seq, int key, int& page) {
+    const int index = key / a.block;
+    page = index < a.width ? a.table[static_cast<size_t>(seq) * a.width + index] : 0;
+    page = page < 0 || page >= a.pool_rows / a.block ? 0 : page;
+    return page * a.block + key % a.block;
+}
+__device__ __forceinline__ float a8_unit(const A8Args& a, const uint8_t* scale, int page, int kvh) {
+    return __uint_as_float(static_cast<uint32_t>(scale[static_cast<size_t>(page) * a.nkv + kvh]) << 23);
+}
+
+// Four neighbouring results of one row, as the caller's type.
+template <int PIECES>
+__device__ __forceinline__ void a8_store4(const A8Args& a, size_t at, float x0, float x1, float x2, float x3) {
+    if constexpr (PIECES == 1) *reinterpret_cast<a8_u32x2*>(static_cast<bf16_t*>(a.out) + at) = a8_u32x2{a8_pack2(x0, x1), a8_pack2(x2, x3)};
+    else *reinterpret_cast<a8_f32x4*>(static_cast<float*>(a.out) + at) = a8_f32x4{x0, x1, x2, x3};
+}
+
+// Eight neighbouring values of a query's head, or zeros.
+template <int PIECES>
+__device__ __forceinline__ void a8_query8(const A8Args& a, size_t at, bool there, a8_frag (&to)[PIECES]) {
+    if constexpr (PIECES == 1) {
+        to[0].raw = there ? *reinterpret_cast<const a8_u32x4*>(static_cast<const bf16_t*>(a.q) + at) : a8_u32x4{0u, 0u, 0u, 0u};
+    } else {
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = there ? static_cast<const float*>(a.q)[at + e] : 0.f;
+        a8_split<PIECES>(x, to);
+    }
+}
+
 // ---- few rows: every wave has keys of its own ------------------------------------------------------------------------------
-// A workgroup takes one block of 32 rows of one key head and one share of the keys; its waves take tiles of 32 keys in turn, each with a running maximum and sum, and meet at the end.
+// A workgroup takes the RB blocks of 16 rows of one request and key head and one share of the keys; its waves take tiles of 32 keys in turn, each with a running maximum and sum, and meet at the end.
 // Keys go from memory into the registers that the product reads (a lane reads 16 bytes of one key: the contraction may go through a head's values in any order, so the
-// queries are laid out to match); values go through a piece of LDS that belongs to the wave, so the loop has no barrier.
-template <int PIECES, int DT>
-__global__ __launch_bounds__(A8_WAVES * PL_WAVE, PIECES * DT >= 8 && DT != 4 ? 1 : 2) void attention_8bit_kernel(A8Args a) {
-    typedef typename A8Type<PIECES>::type T;
-    constexpr int DP = 32 * DT, VROW = DP + a8_pad(DT);
-    constexpr int MEET = 2 * A8_ROWS * (DP + 4) * 4;         // two waves' outputs, behind the loop
-    constexpr int VALUES = A8_WAVES * A8_KEYS * VROW * 2;
+// queries are laid out to match); values go through a piece of LDS that belongs to the wave, so the loop has no barrier.  The next tile's bytes are on their way while a tile is worked on.
+//   S^T = K . Q^T: v_mfma_f32_16x16x32_bf16, twice for 32 keys; a lane has for row lane % 16 the keys 4 (lane / 16) .. + 3 of both.  DQ: the head is padded to 64 DQ values.
+template <int PIECES, int DQ, int RB>
+__global__ __launch_bounds__(A8_WAVES * PL_WAVE, PIECES * RB * DQ >= 6 ? 1 : 2) void attention_8bit_few_kernel(A8Args a) {
+    constexpr int DP = 64 * DQ, VROW = DP + 16;              // (16 more: eight rows read transposed fall on every bank once)
+    constexpr int MROW = DP + 4;
+    constexpr int VALUES = A8_WAVES * A8_KEYS * VROW * 2, MEET = 2 * 16 * MROW * 4;
+    static_assert(MEET <= VALUES, "the waves meet where their values were");
     extern __shared__ __attribute__((aligned(16))) char lds[];
     uint16_t* values = reinterpret_cast<uint16_t*>(lds);
-    int* slots = reinterpret_cast<int*>(lds + (MEET > VALUES ? MEET : VALUES));
+    float* stats = reinterpret_cast<float*>(lds + VALUES);   // [waves][2][rows]
+    int* slots = reinterpret_cast<int*>(stats + A8_WAVES * 2 * 16 * RB);
     float* k_unit = reinterpret_cast<float*>(slots + a.chunk);
     float* v_unit = k_unit + a.chunk;
-    float* stats = v_unit + a.chunk;                         // [waves][2][rows]
+
+    const int tid = threadIdx.x, lane = tid % PL_WAVE, wave = tid / PL_WAVE;
+    const int col = lane % 16, quarter = lane / 16;
+    const int group = a.nq / a.nkv;
+    const int kvh = blockIdx.x % a.nkv, seq = blockIdx.x / a.nkv;
+    if (!a8_brings(a, seq) || a.q_len[seq] * group > 16 * RB) return;
+    const int q_len = a.q_len[seq], start = a.ctx_len[seq] - q_len, rows = q_len * group;
+    const int lo = pl_first_visible(start, a.window), hi = start + q_len;
+    const int shares = a8_shares(lo, hi, a.chunk), share = blockIdx.y;
+    if (share >= shares) return;
+    const int k_base = (lo / a.chunk + share) * a.chunk;
+    const int k_begin = max(lo, k_base), k_end = min(hi, k_base + a.chunk);
+    const int last_from = pl_first_visible(start + q_len - 1, a.window);     // (the last token's first key: no token's is later)
+
+    // Where the keys of the share are, and in what units.  (Keys that no row sees are read at the nearest one's place.)
+    for (int i = tid; i < a.chunk; i += A8_WAVES * PL_WAVE) {
+        int page;
+        slots[i] = a8_slot(a, seq, min(max(k_base + i, k_begin), k_end - 1), page);
+        k_unit[i] = a8_unit(a, a.k_scale, page, kvh);
+        v_unit[i] = a8_unit(a, a.v_scale, page, kvh);
+    }
+
+    // The rows: what a lane reads of a key with its j-th load are the values 64 j + 16 quarter .. + 15, two operands
+    const int q_start = a.q_start[seq];
+    int position[RB], seen_from[RB], out_row[RB];
+    a8_frag qf[RB][2 * DQ][PIECES];
+#pragma unroll
+    for (int b = 0; b < RB; ++b) {
+        const int row = 16 * b + col;
+        const bool live = row < rows;
+        const int token = live ? row / group : 0, head = kvh * group + (live ? row % group : 0);
+        position[b] = start + token;
+        seen_from[b] = pl_first_visible(position[b], a.window);
+        out_row[b] = live ? (q_start + token) * a.nq + head : -1;
+#pragma unroll
+        for (int j = 0; j < 2 * DQ; ++j) {
+            const int at = 64 * (j / 2) + 16 * quarter + 8 * (j % 2);
+            a8_query8<PIECES>(a, static_cast<size_t>(q_start + token) * a.q_stride + static_cast<size_t>(head) * a.d + at, live && at < a.d, qf[b][j]);
+        }
+    }
+    __syncthreads();
+
+    uint16_t* mine = values + wave * A8_KEYS * VROW;
+    a8_f32x4 acc[RB][4 * DQ];
+    float m[RB], l[RB];
+#pragma unroll
+    for (int b = 0; b < RB; ++b) {
+        m[b] = -INFINITY;
+        l[b] = 0.f;
+#pragma unroll
+        for (int t = 0; t < 4 * DQ; ++t) acc[b][t] = a8_f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+
+    // A tile on its way: keys in two halves of 16, values 16 bytes a lane, 4 DQ lanes a key
+    constexpr int VP = 4 * DQ, LOADS = 2 * DQ;
+    a8_u32x4 kraw[LOADS], vraw[LOADS];
+    const size_t row_bytes = static_cast<size_t>(a.nkv) * a.d;
+    const uint8_t *k_from = a.k_pool + static_cast<size_t>(kvh) * a.d, *v_from = a.v_pool + static_cast<size_t>(kvh) * a.d;
+    auto fetch = [&](int base) {
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) {
+            const int at = i * PL_WAVE + lane, piece = at % VP;
+            vraw[i] = a8_u32x4{0u, 0u, 0u, 0u};
+            if (16 * piece < a.d) vraw[i] = *reinterpret_cast<const a8_u32x4*>(v_from + slots[base + at / VP] * row_bytes + 16 * piece);
+        }
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const uint8_t* from = k_from + slots[base + 16 * half + col] * row_bytes;
+#pragma unroll
+            for (int j = 0; j < DQ; ++j) {
+                const int at = 64 * j + 16 * quarter;
+                kraw[half * DQ + j] = a8_u32x4{0u, 0u, 0u, 0u};
+                if (at < a.d) kraw[half * DQ + j] = *reinterpret_cast<const a8_u32x4*>(from + at);
+            }
+        }
+    };
+    // this wave's first and last tiles with keys
+    const int first_tile = (k_begin - k_base) / A8_KEYS, end_tile = pl_ceil_div(k_end - k_base, A8_KEYS);
+    int tile = first_tile + wave;
+    if (tile < end_tile) fetch(tile * A8_KEYS);
+    for (; tile < end_tile; tile += A8_WAVES) {
+        const int base = tile * A8_KEYS, k0 = k_base + base;
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) {
+            const int at = i * PL_WAVE + lane, key = at / VP, piece = at % VP;
+            const float unit = v_unit[base + key];
+            a8_frag to[2];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) to[e / 2].half[e % 2] = a8_widen4(vraw[i][e], unit);
+            // (the first eight of 16 values stand in the row's first half, the others in its second: neighbouring lanes write neighbouring pieces)
+            *reinterpret_cast<a8_u32x4*>(mine + key * VROW + 8 * piece) = to[0].raw;
+            *reinterpret_cast<a8_u32x4*>(mine + key * VROW + DP / 2 + 8 * piece) = to[1].raw;
+        }
+        a8_f32x4 s[RB][2];
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const float unit = k_unit[base + 16 * half + col];
+#pragma unroll
+            for (int b = 0; b < RB; ++b) s[b][half] = a8_f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int j = 0; j < 2 * DQ; ++j) {
+                a8_frag kf;
+                kf.half[0] = a8_widen4(kraw[half * DQ + j / 2][2 * (j % 2)], unit);
+                kf.half[1] = a8_widen4(kraw[half * DQ + j / 2][2 * (j % 2) + 1], unit);
+#pragma unroll
+                for (int b = 0; b < RB; ++b)
+#pragma unroll
+                    for (int p = PIECES - 1; p >= 0; --p) s[b][half] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf.vec, qf[b][j][p].vec, s[b][half], 0, 0, 0);
+            }
+        }
+        if (tile + A8_WAVES < end_tile) fetch((tile + A8_WAVES) * A8_KEYS);
+        const bool whole = k0 >= k_begin && k0 >= last_from && k0 + A8_KEYS <= k_end && k0 + A8_KEYS - 1 <= start;
+        a8_frag pf[RB][PIECES];
+#pragma unroll
+        for (int b = 0; b < RB; ++b) {
+            // (Chosen value by value: elements of a product's result written under a branch have come out as another element here, in the build for 32 bits.)
+            float x[8], top = m[b];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                x[e] = s[b][e / 4][e % 4] * a.scale;
+                if (!whole) {
+                    const int key = k0 + 16 * (e / 4) + 4 * quarter + e % 4;
+                    x[e] = key >= k_begin && key < k_end && key <= position[b] && key >= seen_from[b] ? x[e] : -INFINITY;
+                }
+                top = fmaxf(top, x[e]);
+            }
+            top = fmaxf(top, __shfl_xor(top, 16, PL_WAVE));
+            top = fmaxf(top, __shfl_xor(top, 32, PL_WAVE));
+            const float from = top == -INFINITY ? 0.f : top;
+            const float alpha = __builtin_amdgcn_exp2f(m[b] - from);
+            m[b] = top;
+            float sum = 0.f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                x[e] = __builtin_amdgcn_exp2f(x[e] - from);
+                sum += x[e];
+            }
+            l[b] = l[b] * alpha + sum;
+            a8_split<PIECES>(x, pf[b]);
+#pragma unroll
+            for (int t = 0; t < 4 * DQ; ++t) acc[b][t] *= alpha;
+        }
+        __builtin_amdgcn_wave_barrier();
+        const uint16_t* from = mine + (4 * quarter + col / 4) * VROW + 4 * (col % 4);
+#pragma unroll
+        for (int t = 0; t < 4 * DQ; ++t) {
+            a8_frag vf;
+            vf.half[0] = a8_read_transposed(from + 16 * t);
+            vf.half[1] = a8_read_transposed(from + 16 * VROW + 16 * t);
+#pragma unroll
+            for (int b = 0; b < RB; ++b)
+#pragma unroll
+                for (int p = PIECES - 1; p >= 0; --p) acc[b][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf.vec, pf[b][p].vec, acc[b][t], 0, 0, 0);
+        }
+        __builtin_amdgcn_wave_barrier();
+    }
+
+    // The waves meet: maximum and sum first, then the outputs in halves, always in the same order.
+#pragma unroll
+    for (int b = 0; b < RB; ++b) {
+        l[b] += __shfl_xor(l[b], 16, PL_WAVE);
+        l[b] += __shfl_xor(l[b], 32, PL_WAVE);
+        if (quarter == 0) {
+            stats[(2 * wave) * 16 * RB + 16 * b + col] = m[b];
+            stats[(2 * wave + 1) * 16 * RB + 16 * b + col] = l[b];
+        }
+    }
+    __syncthreads();
+    float* meet = reinterpret_cast<float*>(lds);
+#pragma unroll
+    for (int b = 0; b < RB; ++b) {
+        float top = -INFINITY, total = 0.f;
+#pragma unroll
+        for (int w = 0; w < A8_WAVES; ++w) top = fmaxf(top, stats[2 * w * 16 * RB + 16 * b + col]);
+        const float from = top == -INFINITY ? 0.f : top;
+#pragma unroll
+        for (int w = 0; w < A8_WAVES; ++w)
+            total += stats[(2 * w + 1) * 16 * RB + 16 * b + col] * __builtin_amdgcn_exp2f(stats[2 * w * 16 * RB + 16 * b + col] - from);
+        const float weight = __builtin_amdgcn_exp2f(m[b] - from);
+#pragma unroll
+        for (int t = 0; t < 4 * DQ; ++t) acc[b][t] *= weight;
+#pragma unroll
+        for (int step = A8_WAVES / 2; step > 0; step /= 2) {
+            if (wave >= step && wave < 2 * step && out_row[b] >= 0)
+#pragma unroll
+                for (int t = 0; t < 4 * DQ; ++t) *reinterpret_cast<a8_f32x4*>(meet + ((wave - step) * 16 + col) * MROW + 16 * t + 4 * quarter) = acc[b][t];
+            __syncthreads();
+            if (wave < step && out_row[b] >= 0)
+#pragma unroll
+                for (int t = 0; t < 4 * DQ; ++t) acc[b][t] += *reinterpret_cast<const a8_f32x4*>(meet + (wave * 16 + col) * MROW + 16 * t + 4 * quarter);
+            __syncthreads();
+        }
+        if (wave == 0 && out_row[b] >= 0) {
+            const size_t place = static_cast<size_t>(out_row[b]) * a.chunks + share;
+            if (a.chunks == 1) {
+                if (shares > 1) total = NAN;          // (a context longer than the caller said)
+                const float inv = total != 0.f ? 1.f / total : 0.f;
+#pragma unroll
+                for (int t = 0; t < 4 * DQ; ++t) acc[b][t] *= inv;
+            } else if (quarter == 0) {
+                a.part_ml[2 * place] = top;
+                a.part_ml[2 * place + 1] = total;
+            }
+#pragma unroll
+            for (int t = 0; t < 4 * DQ; ++t) {
+                const int c = 16 * t + 4 * quarter;           // (as the values stood in LDS)
+                const int at = 16 * (c % (DP / 2) / 8) + 8 * (c / (DP / 2)) + c % 8;
+                if (at >= a.d) continue;
+                if (a.chunks == 1) a8_store4<PIECES>(a, static_cast<size_t>(out_row[b]) * a.d + at, acc[b][t][0], acc[b][t][1], acc[b][t][2], acc[b][t][3]);
+                else *reinterpret_cast<a8_f32x4*>(a.part_acc + place * a.d + at) = acc[b][t];
+            }
+        }
+    }
+}
+
+// ---- many rows: every wave has rows of its own -----------------------------------------------------------------------------
+// A workgroup takes NW blocks of 32 rows of one request and key head and one share of the keys, a block a wave.  Tiles of 64 keys come into LDS as bfloat16, two lengths of them: while one is worked on, the bytes of the
+// next (which came into registers a tile earlier) are widened into the other, so what an e4m3 value costs to widen is paid once for all the rows, and a round has one barrier.
+//   S^T = K . Q^T: v_mfma_f32_32x32x16_bf16; a lane has for row lane % 32 the keys 8 (i / 4) + 4 (lane / 32) + i % 4 of 32.  DT: the head is padded to 32 DT values.
+#define A8_TILE 64
+template <int PIECES, int DT, int NW>
+__global__ __launch_bounds__(NW * PL_WAVE, PIECES * DT >= 8 ? 1 : 2) void attention_8bit_many_kernel(A8Args a, int few) {
+    constexpr int DP = 32 * DT, KROW = DP + 8, VROW = DP + (DT % 2 == 0 ? 32 : 0), THREADS = NW * PL_WAVE;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    uint16_t* keys = reinterpret_cast<uint16_t*>(lds);                 // [2][64][KROW]
+    uint16_t* values = keys + 2 * A8_TILE * KROW;                      // [2][64][VROW]
 
     const int tid = threadIdx.x, lane = tid % PL_WAVE, wave = tid / PL_WAVE;
     const int col = lane % 32, half = lane / 32;
     const int group = a.nq / a.nkv;
     const int kvh = blockIdx.x % a.nkv;
     int seq, rb;
-    if (!a8_find(a, blockIdx.x / a.nkv, group, A8_ROWS, seq, rb)) return;
-    const int q_len = a.q_len[seq], ctx = a.ctx_len[seq], start = ctx - q_len;
-    const int first_row = rb * A8_ROWS, rows = min(A8_ROWS, q_len * group - first_row);
-    const int first_token = first_row / group, last_token = (first_row + rows - 1) / group;
-    const int lo = pl_first_visible(start + first_token, a.window), hi = start + last_token + 1;
-    const int share0 = lo / a.chunk, shares = a8_shares(lo, hi, a.chunk);
-    const int share = blockIdx.y;
+    if (!a8_find(a, blockIdx.x / a.nkv, group, 32 * NW, few, seq, rb)) return;
+    const int q_len = a.q_len[seq], start = a.ctx_len[seq] - q_len, q_start = a.q_start[seq];
+    const int first_row = rb * 32 * NW, rows = min(32 * NW, q_len * group - first_row);
+    const int lo = pl_first_visible(start + first_row / group, a.window), hi = start + (first_row + rows - 1) / group + 1;
+    const int shares = a8_shares(lo, hi, a.chunk), share = blockIdx.y;
     if (share >= shares) return;
-    const int k_begin = max(lo, (share0 + share) * a.chunk), k_end = min(hi, (share0 + share + 1) * a.chunk);
-    const int k_base = (share0 + share) * a.chunk;
+    const int k_base = (lo / a.chunk + share) * a.chunk;
+    const int k_begin = max(lo, k_base), k_end = min(hi, k_base + a.chunk);
 
-    // Where the keys of the share are, and in what units.  (Keys that no row sees are read at the last one's place.)
-    for (int i = tid; i < a.chunk; i += A8_WAVES * PL_WAVE) {
-        const int key = min(max(k_base + i, k_begin), k_end - 1);
-        const int index = key / a.block;
-        int page = index < a.width ? a.table[static_cast<size_t>(seq) * a.width + index] : 0;
-        page = page < 0 || page >= a.pool_rows / a.block ? 0 : page;
-        slots[i] = page * a.block + key % a.block;
-        k_unit[i] = __uint_as_float(static_cast<uint32_t>(a.k_scale[static_cast<size_t>(page) * a.nkv + kvh]) << 23);
-        v_unit[i] = __uint_as_float(static_cast<uint32_t>(a.v_scale[static_cast<size_t>(page) * a.nkv + kvh]) << 23);
-    }
-
-    // The rows: piece 2j + e of a lane's keys are the values 32j + 16 half + 8e ..
-    const int row = first_row + col;
-    const bool live = col < rows;
-    const int token = live ? row / group : first_token, head = kvh * group + (live ? row % group : 0);
+    // This wave's rows.
+    const int row = first_row + 32 * wave + col;
+    const bool active = 32 * wave < rows, live = 32 * wave + col < rows;
+    const int token = live ? row / group : (first_row + (active ? 32 * wave : 0)) / group, head = kvh * group + (live ? row % group : 0);
     const int position = start + token, seen_from = pl_first_visible(position, a.window);
+    const int first_pos = start + (first_row + (active ? 32 * wave : 0)) / group, last_pos = start + (first_row + min(32 * wave + 32, rows) - 1) / group;
+    const int wave_from = pl_first_visible(first_pos, a.window), last_from = pl_first_visible(last_pos, a.window);
     a8_frag qf[2 * DT][PIECES];
-    {
-        const T* from = static_cast<const T*>(a.q) + static_cast<size_t>(a.q_start[seq] + token) * a.q_stride + static_cast<size_t>(head) * a.d;
 #pragma unroll
-        for (int j = 0; j < 2 * DT; ++j) {
-            const int at = 32 * (j / 2) + 16 * half + 8 * (j % 2);
-            float x[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = live && at < a.d ? to_float(from[at + e]) : 0.f;
-            a8_split<PIECES>(x, qf[j]);
-        }
+    for (int j = 0; j < 2 * DT; ++j) {
+        const int at = 16 * j + 8 * half;
+        a8_query8<PIECES>(a, static_cast<size_t>(q_start + token) * a.q_stride + static_cast<size_t>(head) * a.d + at, live && at < a.d, qf[j]);
     }
-    __syncthreads();
 
-    uint16_t* mine = values + wave * A8_KEYS * VROW;
+    // A tile on its way: 16 bytes a lane and load, 2 DT lanes a key.
+    constexpr int VP = 2 * DT, LOADS = (A8_TILE * VP + THREADS - 1) / THREADS;
+    a8_u32x4 kraw[LOADS], vraw[LOADS];
+    float kun[LOADS], vun[LOADS];
+    auto fetch = [&](int k0) {
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) {
+            const int at = i * THREADS + tid, piece = at % VP;
+            kraw[i] = vraw[i] = a8_u32x4{0u, 0u, 0u, 0u};
+            kun[i] = vun[i] = 1.f;
+            if (at < A8_TILE * VP && 16 * piece < a.d) {
+                int page;
+                const int slot = a8_slot(a, seq, min(max(k0 + at / VP, k_begin), k_end - 1), page);
+                const size_t from = (static_cast<size_t>(slot) * a.nkv + kvh) * a.d + 16 * piece;
+                kraw[i] = *reinterpret_cast<const a8_u32x4*>(a.k_pool + from);
+                vraw[i] = *reinterpret_cast<const a8_u32x4*>(a.v_pool + from);
+                kun[i] = a8_unit(a, a.k_scale, page, kvh);
+                vun[i] = a8_unit(a, a.v_scale, page, kvh);
+            }
+        }
+    };
+    auto put = [&](int buffer) {
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) {
+            const int at = i * THREADS + tid, key = at / VP, piece = at % VP;
+            if (at >= A8_TILE * VP) continue;
+            a8_frag to[2];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) to[e / 2].half[e % 2] = a8_widen4(kraw[i][e], kun[i]);
+            uint16_t* k_to = keys + (buffer * A8_TILE + key) * KROW + 16 * piece;
+            *reinterpret_cast<a8_u32x4*>(k_to) = to[0].raw;
+            *reinterpret_cast<a8_u32x4*>(k_to + 8) = to[1].raw;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) to[e / 2].half[e % 2] = a8_widen4(vraw[i][e], vun[i]);
+            uint16_t* v_to = values + (buffer * A8_TILE + key) * VROW + 16 * piece;
+            *reinterpret_cast<a8_u32x4*>(v_to) = to[0].raw;
+            *reinterpret_cast<a8_u32x4*>(v_to + 8) = to[1].raw;
+        }
+    };
+
     a8_f32x16 acc[DT];
 #pragma unroll
     for (int t = 0; t < DT; ++t)
@@ -203,179 +488,124 @@ __global__ __launch_bounds__(A8_WAVES * PL_WAVE, PIECES * DT >= 8 && DT != 4 ? 1
         for (int i = 0; i < 16; ++i) acc[t][i] = 0.f;
     float m = -INFINITY, l = 0.f;
 
-    for (int base = wave * A8_KEYS; base < a.chunk; base += A8_WAVES * A8_KEYS) {
-        const int k0 = k_base + base;
-        if (k0 + A8_KEYS <= k_begin || k0 >= k_end) continue;
-        // values: 16 bytes a lane, DP / 16 lanes a key
-        constexpr int VP = DP / 16, VLOADS = A8_KEYS * VP / PL_WAVE;
+    const int k_first = k_begin / A8_TILE * A8_TILE;
+    fetch(k_first);
+    put(0);
+    if (k_first + A8_TILE < k_end) fetch(k_first + A8_TILE);
+    __syncthreads();
+    int buffer = 0;
+    for (int k0 = k_first; k0 < k_end; k0 += A8_TILE, buffer ^= 1) {
+        if (k0 + A8_TILE < k_end) put(buffer ^ 1);
+        if (k0 + 2 * A8_TILE < k_end) fetch(k0 + 2 * A8_TILE);
+        if (active && k0 <= last_pos && k0 + A8_TILE > wave_from) {
+            a8_f32x16 s[2];
+            const uint16_t* k_from = keys + (buffer * A8_TILE + col) * KROW + 8 * half;
 #pragma unroll
-        for (int i = 0; i < VLOADS; ++i) {
-            const int at = i * PL_WAVE + lane, key = at / VP, piece = at % VP;
-            a8_u32x4 raw = {0u, 0u, 0u, 0u};
-            if (16 * piece < a.d) raw = *reinterpret_cast<const a8_u32x4*>(a.v_pool + (static_cast<size_t>(slots[base + key]) * a.nkv + kvh) * a.d + 16 * piece);
-            const float unit = v_unit[base + key];
-            a8_frag to[2];
+            for (int kb = 0; kb < 2; ++kb) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) to[e / 2].half[e % 2] = a8_widen4(raw[e], unit);
-            *reinterpret_cast<a8_u32x4*>(mine + key * VROW + 16 * piece) = to[0].raw;
-            *reinterpret_cast<a8_u32x4*>(mine + key * VROW + 16 * piece + 8) = to[1].raw;
-        }
-        // scores
-        const uint8_t* k_from = a.k_pool + (static_cast<size_t>(slots[base + col]) * a.nkv + kvh) * a.d;
-        const float unit = k_unit[base + col];
-        a8_f32x16 s;
+                for (int i = 0; i < 16; ++i) s[kb][i] = 0.f;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s[i] = 0.f;
+                for (int j = 0; j < 2 * DT; ++j) {
+                    a8_frag kf;
+                    kf.raw = *reinterpret_cast<const a8_u32x4*>(k_from + 32 * kb * KROW + 16 * j);
 #pragma unroll
-        for (int j = 0; j < DT; ++j) {
-            a8_u32x4 raw = {0u, 0u, 0u, 0u};
-            const int at = 32 * j + 16 * half;
-            if (at < a.d) raw = *reinterpret_cast<const a8_u32x4*>(k_from + at);
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                a8_frag kf;
-                kf.half[0] = a8_widen4(raw[2 * e], unit);
-                kf.half[1] = a8_widen4(raw[2 * e + 1], unit);
-#pragma unroll
-                for (int p = PIECES - 1; p >= 0; --p) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf.vec, qf[2 * j + e][p].vec, s, 0, 0, 0);
+                    for (int p = PIECES - 1; p >= 0; --p) s[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf.vec, qf[j][p].vec, s[kb], 0, 0, 0);
+                }
             }
-        }
-        // weights
-        float top = m;
+            const bool whole = k0 >= k_begin && k0 >= last_from && k0 + A8_TILE <= k_end && k0 + A8_TILE - 1 <= first_pos;
+            float top = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const int key = k0 + 8 * (i / 4) + 4 * half + i % 4;
-            s[i] = key >= k_begin && key < k_end && key <= position && key >= seen_from ? s[i] * a.scale : -INFINITY;
-            top = fmaxf(top, s[i]);
-        }
-        top = fmaxf(top, __shfl_xor(top, 32, PL_WAVE));
-        const float base2 = top == -INFINITY ? 0.f : top;
-        const float alpha = __builtin_amdgcn_exp2f(m - base2);
-        m = top;
-        float sum = 0.f;
+            for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            s[i] = __builtin_amdgcn_exp2f(s[i] - base2);
-            sum += s[i];
-        }
-        l = l * alpha + sum;
+                for (int i = 0; i < 16; ++i) {
+                    float x = s[kb][i];
+                    if (!whole) {
+                        const int key = k0 + 32 * kb + 8 * (i / 4) + 4 * half + i % 4;
+                        x = key >= k_begin && key < k_end && key <= position && key >= seen_from ? x : -INFINITY;
+                    }
+                    s[kb][i] = x;
+                    top = fmaxf(top, x);
+                }
+            top = fmaxf(top, __shfl_xor(top, 32, PL_WAVE)) * a.scale;
+            // Weights are taken relative to a maximum that is at most 2^8 off: sums and outputs are scaled anew only where a row's maximum has grown by more.
+            if (__any(top > m + 8.f)) {
+                const float grown = fmaxf(m, top);
+                const float alpha = __builtin_amdgcn_exp2f(m - (grown == -INFINITY ? 0.f : grown));
+                m = grown;
+                l *= alpha;
 #pragma unroll
-        for (int t = 0; t < DT; ++t)
+                for (int t = 0; t < DT; ++t)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) acc[t][i] *= alpha;
-        __builtin_amdgcn_wave_barrier();
-#pragma unroll
-        for (int g = 0; g < 2; ++g) {
-            a8_frag pf[PIECES];
-            float x[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = s[8 * g + e];
-            a8_split<PIECES>(x, pf);
-            const int key = 16 * g + 4 * half + (lane % 16) / 4;
-#pragma unroll
-            for (int t = 0; t < DT; ++t) {
-                const int column = 32 * t + 16 * ((lane / 16) % 2) + 4 * (lane % 4);
-                a8_frag vf;
-                vf.half[0] = a8_read_transposed(mine + key * VROW + column);
-                vf.half[1] = a8_read_transposed(mine + (key + 8) * VROW + column);
-#pragma unroll
-                for (int p = PIECES - 1; p >= 0; --p) acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf.vec, pf[p].vec, acc[t], 0, 0, 0);
+                    for (int i = 0; i < 16; ++i) acc[t][i] *= alpha;
             }
+            const float from = m == -INFINITY ? 0.f : m;
+            float sum = 0.f;
+            const uint16_t* v_from = values + (buffer * A8_TILE + 4 * half + lane % 16 / 4) * VROW + 16 * (lane / 16 % 2) + 4 * (lane % 4);
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                float x[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    x[e] = __builtin_amdgcn_exp2f(fmaf(s[g / 2][8 * (g % 2) + e], a.scale, -from));
+                    sum += x[e];
+                }
+                a8_frag pf[PIECES];
+                a8_split<PIECES>(x, pf);
+#pragma unroll
+                for (int t = 0; t < DT; ++t) {
+                    a8_frag vf;
+                    vf.half[0] = a8_read_transposed(v_from + 16 * g * VROW + 32 * t);
+                    vf.half[1] = a8_read_transposed(v_from + (16 * g + 8) * VROW + 32 * t);
+#pragma unroll
+                    for (int p = PIECES - 1; p >= 0; --p) acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf.vec, pf[p].vec, acc[t], 0, 0, 0);
+                }
+            }
+            l += sum;
         }
-        __builtin_amdgcn_wave_barrier();
+        __syncthreads();
     }
     l += __shfl_xor(l, 32, PL_WAVE);
+    if (!live) return;
 
-    // The waves meet: maximum and sum first, then the outputs in halves, always in the same order.
-    if (half == 0) {
-        stats[(2 * wave) * A8_ROWS + col] = m;
-        stats[(2 * wave + 1) * A8_ROWS + col] = l;
-    }
-    __syncthreads();
-    float top = -INFINITY, total = 0.f;
-#pragma unroll
-    for (int w = 0; w < A8_WAVES; ++w) top = fmaxf(top, stats[2 * w * A8_ROWS + col]);
-    const float base2 = top == -INFINITY ? 0.f : top;
-#pragma unroll
-    for (int w = 0; w < A8_WAVES; ++w) total += stats[(2 * w + 1) * A8_ROWS + col] * __builtin_amdgcn_exp2f(stats[2 * w * A8_ROWS + col] - base2);
-    const float mine2 = __builtin_amdgcn_exp2f(m - base2);
-#pragma unroll
-    for (int t = 0; t < DT; ++t)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) acc[t][i] *= mine2;
-    float* meet = reinterpret_cast<float*>(lds);
-#pragma unroll
-    for (int step = A8_WAVES / 2; step > 0; step /= 2) {
-        if (wave >= step && wave < 2 * step && live)
-#pragma unroll
-            for (int t = 0; t < DT; ++t)
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    *reinterpret_cast<a8_f32x4*>(meet + ((wave - step) * A8_ROWS + col) * (DP + 4) + 32 * t + 8 * i + 4 * half) =
-                        a8_f32x4{acc[t][4 * i], acc[t][4 * i + 1], acc[t][4 * i + 2], acc[t][4 * i + 3]};
-        __syncthreads();
-        if (wave < step && live)
-#pragma unroll
-            for (int t = 0; t < DT; ++t)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const a8_f32x4 other = *reinterpret_cast<const a8_f32x4*>(meet + (wave * A8_ROWS + col) * (DP + 4) + 32 * t + 8 * i + 4 * half);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) acc[t][4 * i + e] += other[e];
-                }
-        __syncthreads();
-    }
-    if (wave != 0 || !live) return;
-
-    const size_t out_row = static_cast<size_t>(a.q_start[seq] + token) * a.nq + head;
+    const size_t out_row = static_cast<size_t>(q_start + token) * a.nq + head, place = out_row * a.chunks + share;
+    float inv = 1.f;
     if (a.chunks == 1) {
-        if (shares > 1) total = NAN;          // (a context longer than the caller said)
-        const float inv = total != 0.f ? 1.f / total : 0.f;
-        T* to = static_cast<T*>(a.out) + out_row * a.d;
-#pragma unroll
-        for (int t = 0; t < DT; ++t)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int at = 32 * t + 8 * i + 4 * half;
-                if (at < a.d) {
-                    if constexpr (PIECES == 1) {
-                        *reinterpret_cast<a8_u32x2*>(to + at) =
-                            a8_u32x2{a8_pack2(acc[t][4 * i] * inv, acc[t][4 * i + 1] * inv), a8_pack2(acc[t][4 * i + 2] * inv, acc[t][4 * i + 3] * inv)};
-                    } else {
-                        *reinterpret_cast<a8_f32x4*>(to + at) = a8_f32x4{acc[t][4 * i] * inv, acc[t][4 * i + 1] * inv, acc[t][4 * i + 2] * inv, acc[t][4 * i + 3] * inv};
-                    }
-                }
-            }
-        return;
-    }
-    const size_t place = out_row * a.chunks + share;
-    if (half == 0) {
-        a.part_ml[2 * place] = top;
-        a.part_ml[2 * place + 1] = total;
+        if (shares > 1) l = NAN;              // (a context longer than the caller said)
+        inv = l != 0.f ? 1.f / l : 0.f;
+    } else if (half == 0) {
+        a.part_ml[2 * place] = m;
+        a.part_ml[2 * place + 1] = l;
     }
 #pragma unroll
     for (int t = 0; t < DT; ++t)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int at = 32 * t + 8 * i + 4 * half;
-            if (at < a.d) *reinterpret_cast<a8_f32x4*>(a.part_acc + place * a.d + at) = a8_f32x4{acc[t][4 * i], acc[t][4 * i + 1], acc[t][4 * i + 2], acc[t][4 * i + 3]};
+            if (at >= a.d) continue;
+            if (a.chunks == 1) a8_store4<PIECES>(a, out_row * a.d + at, acc[t][4 * i] * inv, acc[t][4 * i + 1] * inv, acc[t][4 * i + 2] * inv, acc[t][4 * i + 3] * inv);
+            else *reinterpret_cast<a8_f32x4*>(a.part_acc + place * a.d + at) = a8_f32x4{acc[t][4 * i], acc[t][4 * i + 1], acc[t][4 * i + 2], acc[t][4 * i + 3]};
         }
 }
 
 // ---- shares put together ---------------------------------------------------------------------------------------------------
-// A wave a row and query head: the shares that its block of rows had, in their order.
+// A wave a row and query head: the shares that its block of rows had, in their order.  `per`: rows of a block (0: a request's rows are one block, of at most `few`).
 template <typename T>
-__global__ __launch_bounds__(A8_WAVES * PL_WAVE) void attention_8bit_merge_kernel(A8Args a) {
+__global__ __launch_bounds__(A8_WAVES * PL_WAVE) void attention_8bit_merge_kernel(A8Args a, int few, int per) {
     const int lane = threadIdx.x % PL_WAVE;
     const int group = a.nq / a.nkv;
     const int kvh = blockIdx.x % a.nkv;
-    int seq, rb;
-    if (!a8_find(a, blockIdx.x / a.nkv, group, A8_ROWS, seq, rb)) return;
+    int seq = blockIdx.x / a.nkv, rb = 0;
+    if (per > 0) {
+        if (!a8_find(a, seq, group, per, few, seq, rb)) return;
+    } else if (!a8_brings(a, seq) || a.q_len[seq] * group > few) {
+        return;
+    }
     const int q_len = a.q_len[seq], start = a.ctx_len[seq] - q_len;
-    const int first_row = rb * A8_ROWS, rows = min(A8_ROWS, q_len * group - first_row);
+    const int first_row = rb * per, rows = min(per > 0 ? per : few, q_len * group - first_row);
     const int lo = pl_first_visible(start + first_row / group, a.window), hi = start + (first_row + rows - 1) / group + 1;
     const int all = a8_shares(lo, hi, a.chunk), shares = min(all, a.chunks);
-    for (int r = threadIdx.x / PL_WAVE; r < rows; r += A8_WAVES) {
+    const int threads = A8_WAVES * static_cast<int>(gridDim.y);
+    for (int r = threadIdx.x / PL_WAVE + A8_WAVES * blockIdx.y; r < rows; r += threads) {
         const int row = first_row + r;
         const size_t out_row = static_cast<size_t>(a.q_start[seq] + row / group) * a.nq + kvh * group + row % group;
         const float* ml = a.part_ml + 2 * out_row * a.chunks;
@@ -385,6 +615,7 @@ __global__ __launch_bounds__(A8_WAVES * PL_WAVE) void attention_8bit_merge_kerne
         top = wave_max(top);
         const float base2 = top == -INFINITY ? 0.f : top;
         float total = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
         for (int s = 0; s < shares; ++s) {
             const float w = __builtin_amdgcn_exp2f(ml[2 * s] - base2);
             total += w * ml[2 * s + 1];
@@ -407,55 +638,123 @@ __global__ __launch_bounds__(A8_WAVES * PL_WAVE) void attention_8bit_merge_kerne
     }
 }
 
-template <int PIECES, int DT>
-static int launch_attention(const A8Args& a, long blocks, hipStream_t stream) {
-    constexpr int DP = 32 * DT, VROW = DP + a8_pad(DT);
-    constexpr int MEET = 2 * A8_ROWS * (DP + 4) * 4, VALUES = A8_WAVES * A8_KEYS * VROW * 2;
-    const size_t lds = (MEET > VALUES ? MEET : VALUES) + static_cast<size_t>(a.chunk) * 12 + A8_WAVES * 2 * A8_ROWS * 4;
-    const dim3 grid(static_cast<unsigned>(blocks * a.nkv), static_cast<unsigned>(a.chunks));
-    if (lds > 48 * 1024) {
-        hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&attention_8bit_kernel<PIECES, DT>), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds));
-        PL_REQUIRE(e == hipSuccess, "8-bit attention: %zu bytes of LDS refused: %s", lds, hipGetErrorString(e));
-    }
-    attention_8bit_kernel<PIECES, DT><<<grid, A8_WAVES * PL_WAVE, lds, stream>>>(a);
-    PL_CHECK_LAUNCH("attention_8bit");
+static int a8_lds(const void* kernel, size_t lds) {
+    if (lds <= 48 * 1024) return 0;
+    hipError_t e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds));
+    PL_REQUIRE(e == hipSuccess, "8-bit attention: %zu bytes of LDS refused: %s", lds, hipGetErrorString(e));
+    return 0;
+}
+
+template <int PIECES, int DQ, int RB>
+static int launch_few(const A8Args& a, hipStream_t stream) {
+    const size_t lds = static_cast<size_t>(A8_WAVES) * A8_KEYS * (64 * DQ + 16) * 2 + A8_WAVES * 2 * 16 * RB * 4 + static_cast<size_t>(a.chunk) * 12;
+    if (int e = a8_lds(reinterpret_cast<const void*>(&attention_8bit_few_kernel<PIECES, DQ, RB>), lds)) return e;
+    const unsigned blocks = static_cast<unsigned>(a.S) * a.nkv;
+    attention_8bit_few_kernel<PIECES, DQ, RB><<<dim3(blocks, a.chunks), A8_WAVES * PL_WAVE, lds, stream>>>(a);
+    PL_CHECK_LAUNCH("attention_8bit_few");
     if (a.chunks > 1) {
-        attention_8bit_merge_kernel<typename A8Type<PIECES>::type><<<static_cast<unsigned>(blocks * a.nkv), A8_WAVES * PL_WAVE, 0, stream>>>(a);
+        attention_8bit_merge_kernel<typename A8Type<PIECES>::type><<<dim3(blocks, RB), A8_WAVES * PL_WAVE, 0, stream>>>(a, 16 * RB, 0);
         PL_CHECK_LAUNCH("attention_8bit_merge");
     }
     return 0;
 }
 
+template <int PIECES, int DQ>
+static int launch_few(const A8Args& a, int rows, hipStream_t stream) {
+    constexpr int MOST = A8Few<PIECES, DQ>::BLOCKS;
+    if (rows <= 16 || MOST == 1) return launch_few<PIECES, DQ, 1>(a, stream);
+    if constexpr (MOST >= 2)
+        if (rows <= 32 || MOST == 2) return launch_few<PIECES, DQ, 2>(a, stream);
+    if constexpr (MOST >= 4) {
+        if (rows <= 48) return launch_few<PIECES, DQ, 3>(a, stream);
+        return launch_few<PIECES, DQ, 4>(a, stream);
+    }
+    return 0;
+}
+
 template <int PIECES>
-static int launch_attention(const A8Args& a, long blocks, hipStream_t stream) {
-    switch (pl_ceil_div(a.d, 32)) {
-        case 1: return launch_attention<PIECES, 1>(a, blocks, stream);
-        case 2: return launch_attention<PIECES, 2>(a, blocks, stream);
-        case 3: return launch_attention<PIECES, 3>(a, blocks, stream);
-        case 4: return launch_attention<PIECES, 4>(a, blocks, stream);
-        case 5:
-        case 6: return launch_attention<PIECES, 6>(a, blocks, stream);
-        default: return launch_attention<PIECES, 8>(a, blocks, stream);
+static int launch_few(const A8Args& a, int rows, hipStream_t stream) {
+    switch (pl_ceil_div(a.d, 64)) {
+        case 1: return launch_few<PIECES, 1>(a, rows, stream);
+        case 2: return launch_few<PIECES, 2>(a, rows, stream);
+        case 3: return launch_few<PIECES, 3>(a, rows, stream);
+        default: return launch_few<PIECES, 4>(a, rows, stream);
     }
 }
 
-extern "C" int pl_paged_attention_8bit(const void* q, int q_stride, void* out, const void* q_start, const void* q_len, const void* ctx_len, int S, int n, int max_q_len,
-                                       const void* table, int width, int block, int pool_rows, const void* k_pool, const void* v_pool, const void* k_scale,
-                                       const void* v_scale, int nq, int nkv, int d, float scale, int window, int chunk, int chunks, void* part_acc, void* part_ml, int dtype,
-                                       void* stream) {
-    PL_REQUIRE(d >= 16 && d <= 256 && d % 16 == 0, "8-bit attention: head size %d, the kernel takes multiples of 16 up to 256", d);
-    PL_REQUIRE(nkv >= 1 && nq >= nkv && nq % nkv == 0, "8-bit attention: %d query heads over %d key heads", nq, nkv);
-    PL_REQUIRE(S >= 1 && n >= 1 && max_q_len >= 1 && width >= 1 && block >= 1 && pool_rows >= block, "8-bit attention: %d requests, %d rows, %d of one request, tables of %d pages of %d, %d rows",
-               S, n, max_q_len, width, block, pool_rows);
-    PL_REQUIRE(chunk >= A8_KEYS && chunk % A8_KEYS == 0 && chunk <= 2048 && chunks >= 1 && chunks < 65536 && (chunks == 1 || (part_acc && part_ml)), "8-bit attention: %d shares of %d keys", chunks, chunk);
-    const A8Args a{q, q_stride, out, static_cast<const int*>(q_start), static_cast<const int*>(q_len), static_cast<const int*>(ctx_len), S, static_cast<const int*>(table), width, block, pool_rows,
-                   static_cast<const uint8_t*>(k_pool), static_cast<const uint8_t*>(v_pool), static_cast<const uint8_t*>(k_scale), static_cast<const uint8_t*>(v_scale),
-                   nq, nkv, d, scale * 1.4426950408889634f, window, n, chunk, chunks, static_cast<float*>(part_acc), static_cast<float*>(part_ml)};
-    const int group = nq / nkv;
+template <int PIECES, int DT, int NW>
+static int launch_many(const A8Args& a, int few, long blocks, hipStream_t stream) {
+    const size_t lds = 2 * static_cast<size_t>(A8_TILE) * (32 * DT + 8 + 32 * DT + (DT % 2 == 0 ? 32 : 0)) * 2;
+    if (int e = a8_lds(reinterpret_cast<const void*>(&attention_8bit_many_kernel<PIECES, DT, NW>), lds)) return e;
+    PL_REQUIRE(blocks * a.nkv < (1l << 31), "8-bit attention: %ld blocks of rows are too many for a launch", blocks);
+    attention_8bit_many_kernel<PIECES, DT, NW><<<dim3(static_cast<unsigned>(blocks * a.nkv), a.chunks), NW * PL_WAVE, lds, stream>>>(a, few);
+    PL_CHECK_LAUNCH("attention_8bit_many");
+    if (a.chunks > 1) {
+        attention_8bit_merge_kernel<typename A8Type<PIECES>::type><<<dim3(static_cast<unsigned>(blocks * a.nkv), 4 * NW), A8_WAVES * PL_WAVE, 0, stream>>>(a, few, 32 * NW);
+        PL_CHECK_LAUNCH("attention_8bit_merge");
+    }
+    return 0;
+}
+
+template <int PIECES, int DT>
+static int launch_many(const A8Args& a, int few, int max_q_len, hipStream_t stream) {
+    constexpr int NW = PIECES * DT >= 8 ? 4 : 8;
+    const int group = a.nq / a.nkv;
     // blocks of rows: one a request for what is left over, and the whole ones
-    const long most = static_cast<long>(S) * pl_ceil_div(max_q_len * group, A8_ROWS);
-    const long all = S + static_cast<long>(n) * group / A8_ROWS;
-    const long blocks = most < all ? most : all;
-    PL_REQUIRE(blocks * nkv < (1l << 31), "8-bit attention: %ld blocks of rows are too many for a launch", blocks);
-    return dtype == PL_DTYPE_F32 ? launch_attention<3>(a, blocks, static_cast<hipStream_t>(stream)) : launch_attention<1>(a, blocks, static_cast<hipStream_t>(stream));
+    const long most = static_cast<long>(a.S) * ((static_cast<long>(max_q_len) * group + 32 * NW - 1) / (32 * NW)), all = a.S + static_cast<long>(a.n) * group / (32 * NW);
+    return launch_many<PIECES, DT, NW>(a, few, most < all ? most : all, stream);
+}
+
+template <int PIECES>
+static int launch_many(const A8Args& a, int few, int max_q_len, hipStream_t stream) {
+    switch (pl_ceil_div(a.d, 32)) {
+        case 1: return launch_many<PIECES, 1>(a, few, max_q_len, stream);
+        case 2: return launch_many<PIECES, 2>(a, few, max_q_len, stream);
+        case 3: return launch_many<PIECES, 3>(a, few, max_q_len, stream);
+        case 4: return launch_many<PIECES, 4>(a, few, max_q_len, stream);
+        case 5:
+        case 6: return launch_many<PIECES, 6>(a, few, max_q_len, stream);
+        default: return launch_many<PIECES, 8>(a, few, max_q_len, stream);
+    }
+}
+
+// The most rows (tokens times query heads a key head) of a request that the kernel of few rows takes.
+extern "C" int pl_paged_attention_8bit_few(int d, int dtype) {
+    const int dq = pl_ceil_div(d, 64);
+    if (dtype == PL_DTYPE_F32) return 16 * (dq == 1 ? A8Few<3, 1>::BLOCKS : dq == 2 ? A8Few<3, 2>::BLOCKS : A8Few<3, 3>::BLOCKS);
+    return 16 * (dq <= 2 ? A8Few<1, 2>::BLOCKS : A8Few<1, 3>::BLOCKS);
+}
+
+// `few_rows`, `many_rows`: the most rows of a request that goes to the kernel of few rows, or 0, and the most of one that goes to the kernel of many, or 0; each has shares of its own size.
+extern "C" int pl_paged_attention_8bit(const void* q, int q_stride, void* out, const void* q_start, const void* q_len, const void* ctx_len, int S, int n, int max_q_len, int min_q_len,
+                                       const void* table, int width, int block, int pool_rows, const void* k_pool, const void* v_pool, const void* k_scale,
+                                       const void* v_scale, int nq, int nkv, int d, float scale, int window, int few_chunk, int few_chunks, int many_chunk, int many_chunks,
+                                       void* part_acc, void* part_ml, int dtype, void* stream) {
+    PL_REQUIRE(d >= 16 && d <= 256 && d % 16 == 0, "8-bit attention: head size %d, the kernels take multiples of 16 up to 256", d);
+    PL_REQUIRE(nkv >= 1 && nq >= nkv && nq % nkv == 0, "8-bit attention: %d query heads over %d key heads", nq, nkv);
+    PL_REQUIRE(S >= 1 && n >= 1 && max_q_len >= 1 && min_q_len <= max_q_len && width >= 1 && block >= 1 && pool_rows >= block,
+               "8-bit attention: %d requests, %d rows, %d to %d of one request, tables of %d pages of %d, %d rows", S, n, min_q_len, max_q_len, width, block, pool_rows);
+    PL_REQUIRE(static_cast<long>(n) * nq < (1l << 31) && static_cast<long>(S) * nkv < (1l << 31), "8-bit attention: %d rows of %d heads, %d requests are too many for a launch", n, nq, S);
+    PL_REQUIRE(few_chunk >= A8_KEYS && few_chunk % A8_KEYS == 0 && few_chunk <= 4096 && few_chunks >= 1 && few_chunks < 65536 && (few_chunks == 1 || (part_acc && part_ml)),
+               "8-bit attention: %d shares of %d keys", few_chunks, few_chunk);
+    PL_REQUIRE(many_chunk >= A8_TILE && many_chunk % A8_TILE == 0 && many_chunks >= 1 && many_chunks < 65536 && (many_chunks == 1 || (part_acc && part_ml)),
+               "8-bit attention: %d shares of %d keys", many_chunks, many_chunk);
+    A8Args a{q, q_stride, out, static_cast<const int*>(q_start), static_cast<const int*>(q_len), static_cast<const int*>(ctx_len), S, static_cast<const int*>(table), width, block, pool_rows,
+             static_cast<const uint8_t*>(k_pool), static_cast<const uint8_t*>(v_pool), static_cast<const uint8_t*>(k_scale), static_cast<const uint8_t*>(v_scale),
+             nq, nkv, d, scale * 1.4426950408889634f, window, n, few_chunk, few_chunks, static_cast<float*>(part_acc), static_cast<float*>(part_ml)};
+    const int few = pl_paged_attention_8bit_few(d, dtype);
+    const long group = nq / nkv, longest = max_q_len * group;
+    const hipStream_t on = static_cast<hipStream_t>(stream);
+    const bool f32 = dtype == PL_DTYPE_F32;
+    if (longest > few) {
+        a.chunk = many_chunk;
+        a.chunks = many_chunks;
+        if (int e = f32 ? launch_many<3>(a, few, max_q_len, on) : launch_many<1>(a, few, max_q_len, on)) return e;
+    }
+    if (min_q_len * group <= few) {
+        a.chunk = few_chunk;
+        a.chunks = few_chunks;
+        return f32 ? launch_few<3>(a, static_cast<int>(min(longest, static_cast<long>(few))), on) : launch_few<1>(a, static_cast<int>(min(longest, static_cast<long>(few))), on);
+    }
+    return 0;
 }

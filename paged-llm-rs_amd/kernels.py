@@ -123,7 +123,8 @@ def _signatures(lib) -> None:
         "pl_sandwich_step": [p, p, p, p, f, p, p, f, p, i, p, i, i, i, p],
         "pl_step_tables": [p, p, i, p, i, i, p, i, i, p, p, p, p, p, p],
         "pl_qk_norm_rope_kv_write_8bit": [p, p, i, p, p, i, f, p, p, i, i, i, p, p, i, i, p, p, p, p, i, i, i, i, i, p],
-        "pl_paged_attention_8bit": [p, i, p, p, p, p, i, i, i, p, i, i, i, p, p, p, p, i, i, i, f, i, i, i, p, p, i, p],
+        "pl_paged_attention_8bit": [p, i, p, p, p, p, i, i, i, i, p, i, i, i, p, p, p, p, i, i, i, f, i, i, i, i, i, p, p, i, p],
+        "pl_paged_attention_8bit_few": [i, i],
         "pl_bigram_add": [p, p, p, p, p, p, p, p, p, p, p, i, ctypes.c_longlong, ctypes.c_longlong, ctypes.c_longlong, i, i, p],
     }
     for name, argtypes in table.items():
@@ -3037,11 +3038,13 @@ def qk_norm_rope_kv_write_8bit(qkv: torch.Tensor, q: torch.Tensor | None, q_gain
 
 
 def shares_8bit(n: int, requests: int, max_ctx: int, nq: int, nkv: int, window: int = 0) -> tuple:
-    """(keys a share, shares) of the 8-bit attention's few-row kernel."""
-    reach = max_ctx if window <= 0 else min(max_ctx, window + 32)
-    chunk = 512
-    shares = (max_ctx + chunk - 1) // chunk
-    return chunk, min(shares, reach // chunk + 2) if window > 0 else shares
+    """(keys a share, shares) of the 8-bit attention's kernel of few rows, and the same of its kernel of many."""
+    few = many = 512
+    # (under a window a block of rows reaches over the window and its own tokens)
+    within = lambda chunk: min((max_ctx + chunk - 1) // chunk, (window + 256) // chunk + 2) if window > 0 else (max_ctx + chunk - 1) // chunk  # noqa: E731
+    if n * nq > 256 * 512:
+        many = (max_ctx + 63) // 64 * 64
+    return few, within(few), many, within(many)
 
 
 def paged_attention_8bit(q: torch.Tensor, q_row_stride: int, out: torch.Tensor, q_start: torch.Tensor, q_len: torch.Tensor, ctx_len: torch.Tensor, max_q_len: int,
@@ -3076,14 +3079,15 @@ def paged_attention_8bit(q: torch.Tensor, q_row_stride: int, out: torch.Tensor, 
         raise TensorError(f"scores scaled by {scale}, which has to be finite and above zero")
     if q_row_stride % 8 or not in_pieces(q, out):
         raise TensorError("query rows and outputs for an 8-bit cache begin at whole 16 bytes")
-    chunk, chunks = shares_8bit(n, S, int(max_ctx), nq, nkv, int(window or 0))
+    few, few_shares, many, many_shares = shares_8bit(n, S, int(max_ctx), nq, nkv, int(window or 0))
+    chunks = max(few_shares, many_shares)
     acc = ml = 0
     if chunks > 1:
         room = torch.empty(n * nq * chunks * (d + 2), dtype=torch.float32, device=q.device)
         acc = room.data_ptr()
         ml = acc + 4 * n * nq * chunks * d
     _check(library().pl_paged_attention_8bit(
-        q.data_ptr(), q_row_stride, out.data_ptr(), q_start.data_ptr(), q_len.data_ptr(), ctx_len.data_ptr(), S, n, max_q_len, block_table.data_ptr(),
+        q.data_ptr(), q_row_stride, out.data_ptr(), q_start.data_ptr(), q_len.data_ptr(), ctx_len.data_ptr(), S, n, max_q_len, min_q_len, block_table.data_ptr(),
         block_table.shape[1], block_size, rows, k_pool.data_ptr(), v_pool.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), nq, nkv, d, scale, int(window or 0),
-        chunk, chunks, acc, ml, code, _stream()))
+        few, few_shares, many, many_shares, acc, ml, code, _stream()))
     return out
