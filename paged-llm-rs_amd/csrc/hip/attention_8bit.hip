@@ -175,7 +175,7 @@ __device__ __forceinline__ void a8_query8(const A8Args& a, size_t at, bool there
 // queries are laid out to match); values go through a piece of LDS that belongs to the wave, so the loop has no barrier.  The next tile's bytes are on their way while a tile is worked on.
 //   S^T = K . Q^T: v_mfma_f32_16x16x32_bf16, twice for 32 keys; a lane has for row lane % 16 the keys 4 (lane / 16) .. + 3 of both.  DQ: the head is padded to 64 DQ values.
 template <int PIECES, int DQ, int RB>
-__global__ __launch_bounds__(A8_WAVES * PL_WAVE, PIECES * RB * DQ >= 6 ? 1 : 2) void attention_8bit_few_kernel(A8Args a) {
+__global__ __launch_bounds__(A8_WAVES * PL_WAVE, PIECES * RB * DQ > 6 || (PIECES == 3 && RB * DQ > 1) ? 1 : 2) void attention_8bit_few_kernel(A8Args a) {
     constexpr int DP = 64 * DQ, VROW = DP + 16;              // (16 more: eight rows read transposed fall on every bank once)
     constexpr int MROW = DP + 4;
     constexpr int VALUES = A8_WAVES * A8_KEYS * VROW * 2, MEET = 2 * 16 * MROW * 4;

@@ -9,6 +9,7 @@
 
 #define P8_LARGEST_SEQS 8192      // two words of LDS a request: 64 KB
 #define P8_TABLE_THREADS 256
+#define P8_HEADS 4                // query heads a group of lanes
 
 // ---- block tables and slots ---------------------------------------------------------------------------------------------
 // Request s brings q_len[s] tokens, its context behind the step is ctx_len[s]; it holds ceil((ctx - q) / block) pages and needs ceil(ctx / block).  Where new pages
@@ -161,52 +162,101 @@ __device__ __forceinline__ void p8_load8(const T* from, float (&to)[8]) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) to[e] = to_float(p.v[e]);
 }
+__device__ __forceinline__ void p8_gain8(const P8Write& a, bool key, int at, float (&to)[8]) {
+    const void* gain = key ? a.k_gain : a.q_gain;
+    if (a.gain_dtype == PL_DTYPE_F32) p8_load8(static_cast<const float*>(gain) + at, to);
+    else p8_load8(static_cast<const bf16_t*>(gain) + at, to);
+}
 
-__device__ __forceinline__ float p8_gain(const P8Write& a, bool key, int at) { return load_as_float(key ? a.k_gain : a.q_gain, a.gain_dtype, at); }
+// Eight values (`chunk` of the row) of head `head` of row `row`, normed and turned where they are a query's or a key's.  All LPR lanes of a row call this together.  Everything that is read
+// is asked for before the first sum, so a row costs one wait.
+// PIECES: the rotation turns halves of whole pieces, so a piece's partners are another lane's piece and its angles a piece of the tables (or nothing is turned); any other rotation looks its
+// partners up one by one, which takes two and a half times the registers and so has a kernel of its own.
+// What a lane needs of a row beside its values: the same for all heads of queries, or of keys, of the row.
+template <int LPR, bool PIECES>
+struct P8Turn {
+    float g[8], c[8], s[8];
+    size_t angle;
+    bool here, key, plain, turned, low;
 
-// Eight values (`chunk` of the row) of head `head` of row `row`, normed and turned where they are a query's or a key's.  All LPR lanes of a row call this together.
-template <typename T, int LPR>
-__device__ __forceinline__ void p8_prepare(const P8Write& a, int row, int head, int chunk, bool live, float (&x)[8]) {
-    const T* base = static_cast<const T*>(a.qkv) + (static_cast<size_t>(row) * (a.nq + 2 * a.nkv) + head) * a.d;
-    const bool here = live && chunk * 8 < a.d;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = 0.f;
-    if (here) p8_load8(base + chunk * 8, x);
-    if (head >= a.nq + a.nkv) return;
-    const bool key = head >= a.nq;
-    float rinv = 1.f;
-    if (a.q_gain != nullptr) {
-        float ss = 0.f;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], ss);
-#pragma unroll
-        for (int off = LPR / 2; off > 0; off >>= 1) ss += __shfl_xor(ss, off, PL_WAVE);
-        rinv = 1.f / sqrtf(ss / static_cast<float>(a.d) + a.eps);
-        if (here)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = x[e] * rinv * p8_gain(a, key, chunk * 8 + e);
-    }
-    if (a.rot == 0 || !here) return;
-    const int half = a.rot / 2;
-    const int angle = min(max(a.positions[row], 0), a.angles - 1);
-    const float *c = a.cos + static_cast<size_t>(angle) * half, *s = a.sin + static_cast<size_t>(angle) * half;
-    float old[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) old[e] = x[e];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        const int i = chunk * 8 + e;
-        if (i >= a.rot) continue;
-        if (a.neighbours) {
-            x[e] = e % 2 == 0 ? old[e] * c[i / 2] - old[e ^ 1] * s[i / 2] : old[e] * c[i / 2] + old[e ^ 1] * s[i / 2];
-        } else {
-            const bool low = i < half;
-            const int at = low ? i : i - half, other = low ? i + half : i - half;
-            float p = to_float(base[other]);
-            if (a.q_gain != nullptr) p = p * rinv * p8_gain(a, key, other);
-            x[e] = low ? old[e] * c[at] - p * s[at] : old[e] * c[at] + p * s[at];
+    __device__ __forceinline__ P8Turn(const P8Write& a, int row, int head, int chunk, bool live) {
+        const int half = a.rot / 2, first = chunk * 8;
+        here = live && first < a.d;
+        key = head >= a.nq;
+        plain = head >= a.nq + a.nkv;
+        turned = !plain && first < a.rot;
+        low = first < half;
+        angle = static_cast<size_t>(a.rot > 0 && !plain ? min(max(a.positions[row], 0), a.angles - 1) : 0) * half;
+        if (!plain && here && a.q_gain != nullptr) p8_gain8(a, key, first, g);
+        if (PIECES && turned && here) {
+            p8_load8(a.cos + angle + (low ? first : first - half), c);
+            p8_load8(a.sin + angle + (low ? first : first - half), s);
         }
     }
+
+    // Eight values of the row that begins at `base`, normed and turned.  All LPR lanes of a row call this together.
+    template <typename T>
+    __device__ __forceinline__ void apply(const P8Write& a, const T* base, int chunk, float (&x)[8]) const {
+        if (plain) return;
+        const int half = a.rot / 2, first = chunk * 8;
+        float rinv = 1.f;
+        if (a.q_gain != nullptr) {
+            float ss = 0.f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], ss);
+#pragma unroll
+            for (int off = LPR / 2; off > 0; off >>= 1) ss += __shfl_xor(ss, off, PL_WAVE);
+            rinv = 1.f / sqrtf(ss / static_cast<float>(a.d) + a.eps);
+            if (here)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[e] = x[e] * rinv * g[e];
+        }
+        if (a.rot == 0) return;
+        if constexpr (PIECES) {
+            const int lane = threadIdx.x % PL_WAVE, other = low ? lane + half / 8 : lane - half / 8;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float p = __shfl(x[e], other, PL_WAVE);
+                if (turned && here) x[e] = low ? x[e] * c[e] - p * s[e] : x[e] * c[e] + p * s[e];
+            }
+        } else {
+            if (!here || !turned) return;
+            float old[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) old[e] = x[e];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int i = first + e;
+                if (i >= a.rot) continue;
+                if (a.neighbours) {
+                    const float ci = a.cos[angle + i / 2], si = a.sin[angle + i / 2];
+                    x[e] = e % 2 == 0 ? old[e] * ci - old[e ^ 1] * si : old[e] * ci + old[e ^ 1] * si;
+                } else {
+                    const bool lower = i < half;
+                    const int at = lower ? i : i - half, other = lower ? i + half : i - half;
+                    float p = to_float(base[other]);
+                    if (a.q_gain != nullptr) p = p * rinv * load_as_float(key ? a.k_gain : a.q_gain, a.gain_dtype, other);
+                    x[e] = lower ? old[e] * a.cos[angle + at] - p * a.sin[angle + at] : old[e] * a.cos[angle + at] + p * a.sin[angle + at];
+                }
+            }
+        }
+    }
+};
+
+template <typename T>
+__device__ __forceinline__ const T* p8_row(const P8Write& a, int row, int head) {
+    return static_cast<const T*>(a.qkv) + (static_cast<size_t>(row) * (a.nq + 2 * a.nkv) + head) * a.d;
+}
+
+// Eight values (`chunk` of the row) of head `head` of row `row`, normed and turned where they are a query's or a key's.
+template <typename T, int LPR, bool PIECES>
+__device__ __forceinline__ void p8_prepare(const P8Write& a, int row, int head, int chunk, float (&x)[8]) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = 0.f;
+    const T* base = p8_row<T>(a, row, head);
+    if (chunk * 8 < a.d) p8_load8(base + chunk * 8, x);
+    const P8Turn<LPR, PIECES> turn(a, row, head, chunk, true);
+    turn.apply(a, base, chunk, x);
 }
 
 __device__ __forceinline__ bool p8_finite(float v) { return (__float_as_uint(v) & 0x7f800000u) != 0x7f800000u; }
@@ -243,33 +293,35 @@ __device__ __forceinline__ void p8_values8(uint2 bytes, float (&x)[8]) {
     }
 }
 
-template <typename T, int LPR, int WAVES>
-__device__ __forceinline__ void p8_run(const P8Write& a, int first, int head, bool keys, float* scratch) {
+template <typename T, int LPR, int WAVES, bool PIECES>
+__device__ __forceinline__ void p8_run(const P8Write& a, int first, int slot, int head, bool keys, float* scratch) {
     constexpr int ROWS = WAVES * PL_WAVE / LPR;         // rows at a time
     const int lane_row = threadIdx.x / LPR, chunk = threadIdx.x % LPR;
-    const int slot = a.slots[first];
     const int page = slot / a.block, off = slot % a.block;
-    int count = min(a.block - off, a.n - first);
-    for (int base = 0; base < count; base += PL_WAVE) {
-        const int i = base + static_cast<int>(threadIdx.x % PL_WAVE);
-        const uint64_t other = __ballot(i < count && a.slots[first + min(i, count - 1)] != slot + i);
-        if (other != 0) {
-            count = base + __ffsll(static_cast<unsigned long long>(other)) - 1;
-            break;
-        }
-    }
     const int source = keys ? a.nq + head : a.nq + a.nkv + head;
     uint8_t* pool = keys ? a.k_pool : a.v_pool;
     uint8_t* scale = (keys ? a.k_scale : a.v_scale) + static_cast<size_t>(page) * a.nkv + head;
     const size_t row_bytes = static_cast<size_t>(a.nkv) * a.d;
     uint8_t* rows = pool + static_cast<size_t>(page) * a.block * row_bytes + static_cast<size_t>(head) * a.d;
+    // The first rows are read before it is known how many are the run's: that costs a wait of its own.
+    const int most = min(a.block - off, a.n - first);
     const int before = off > 0 ? *scale : 0;
-
     float x[8], top = 0.f;
+    p8_prepare<T, LPR, PIECES>(a, first + min(lane_row, most - 1), source, chunk, x);
+    int count = most;
+    for (int base = 0; base < most; base += PL_WAVE) {
+        const int i = base + static_cast<int>(threadIdx.x % PL_WAVE);
+        const uint64_t other = __ballot(i < most && a.slots[first + min(i, most - 1)] != slot + i);
+        if (other != 0) {
+            count = base + __ffsll(static_cast<unsigned long long>(other)) - 1;
+            break;
+        }
+    }
     for (int r = 0; r < count; r += ROWS) {
-        p8_prepare<T, LPR>(a, first + min(r + lane_row, count - 1), source, chunk, true, x);
+        if (r > 0) p8_prepare<T, LPR, PIECES>(a, first + min(r + lane_row, count - 1), source, chunk, x);
+        if (r + lane_row < count)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) top = fmaxf(top, p8_finite(x[e]) ? fabsf(x[e]) : 0.f);
+            for (int e = 0; e < 8; ++e) top = fmaxf(top, p8_finite(x[e]) ? fabsf(x[e]) : 0.f);
     }
     top = wave_max(top);
     if (WAVES > 1) {
@@ -290,14 +342,14 @@ __device__ __forceinline__ void p8_run(const P8Write& a, int first, int head, bo
         }
     }
     for (int r = 0; r < count; r += ROWS) {
-        if (count > ROWS) p8_prepare<T, LPR>(a, first + min(r + lane_row, count - 1), source, chunk, true, x);
+        if (count > ROWS) p8_prepare<T, LPR, PIECES>(a, first + min(r + lane_row, count - 1), source, chunk, x);
         if (r + lane_row < count && chunk * 8 < a.d) *reinterpret_cast<uint2*>(rows + (off + r + lane_row) * row_bytes + chunk * 8) = p8_round8(x, power);
     }
     if (threadIdx.x == 0) *scale = static_cast<uint8_t>(power);
 }
 
 // Workgroups: first nkv * 2 a tile of `tile` rows for keys and values, then those of the queries.
-template <typename T, int LPR, int WAVES>
+template <typename T, int LPR, int WAVES, bool PIECES>
 __global__ __launch_bounds__(WAVES * PL_WAVE) void write_8bit_kernel(P8Write a, int tile) {
     __shared__ float scratch[WAVES];
     constexpr int ROWS = WAVES * PL_WAVE / LPR;
@@ -305,38 +357,55 @@ __global__ __launch_bounds__(WAVES * PL_WAVE) void write_8bit_kernel(P8Write a, 
     const long of_pages = static_cast<long>(tiles) * pairs;
     if (blockIdx.x < of_pages) {
         const int t = blockIdx.x / pairs, pair = blockIdx.x % pairs;
-        const int end = min((t + 1) * tile, a.n);
-        for (int r = t * tile; r < end; ++r) {
-            const int slot = a.slots[r];
-            if (slot < 0 || slot >= a.pool_rows) continue;
-            if (r > 0 && slot % a.block != 0 && a.slots[r - 1] == slot - 1) continue;
-            p8_run<T, LPR, WAVES>(a, r, pair / 2, pair % 2 == 0, scratch);
+        // the first rows of runs, found by every wave for itself
+        const int r = t * tile + static_cast<int>(threadIdx.x % PL_WAVE);
+        const bool mine = r < min((t + 1) * tile, a.n);
+        const int slot = mine ? a.slots[r] : -1, before = mine && r > 0 ? a.slots[r - 1] : -2;
+        uint64_t runs = __ballot(slot >= 0 && slot < a.pool_rows && (slot % a.block == 0 || before != slot - 1));
+        for (; runs != 0; runs &= runs - 1) {
+            const int which = __ffsll(static_cast<unsigned long long>(runs)) - 1;
+            p8_run<T, LPR, WAVES, PIECES>(a, t * tile + which, __builtin_amdgcn_readfirstlane(__shfl(slot, which, PL_WAVE)), pair / 2, pair % 2 == 0, scratch);
         }
         return;
     }
-    // (row, head) pairs of the queries, ROWS a workgroup
+    // The queries: P8_HEADS heads of a row a group of lanes, which share its angles and gains.
     const int i = static_cast<int>(blockIdx.x - of_pages) * ROWS + static_cast<int>(threadIdx.x / LPR);
-    const int chunk = threadIdx.x % LPR;
-    const bool live = i < a.n * a.nq;
-    const int row = live ? i / a.nq : 0, head = live ? i % a.nq : 0;
-    float x[8];
-    p8_prepare<T, LPR>(a, row, head, chunk, live, x);
-    if (!live || chunk * 8 >= a.d || a.positions[row] < 0) return;
+    const int chunk = threadIdx.x % LPR, blocks = pl_ceil_div(a.nq, P8_HEADS);
+    const bool live = i < a.n * blocks && chunk * 8 < a.d;
+    const int row = i < a.n * blocks ? i / blocks : 0, head = i < a.n * blocks ? i % blocks * P8_HEADS : 0;
+    float x[P8_HEADS][8];
+#pragma unroll
+    for (int h = 0; h < P8_HEADS; ++h) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[h][e] = 0.f;
+        if (live && head + h < a.nq) p8_load8(p8_row<T>(a, row, head + h) + chunk * 8, x[h]);
+    }
+    const P8Turn<LPR, PIECES> turn(a, row, head, chunk, live);
+    const bool written = live && a.positions[row] >= 0;
     struct __attribute__((aligned(16))) Piece {
         T v[8];
     } out;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) out.v[e] = from_float<T>(x[e]);
-    *reinterpret_cast<Piece*>(static_cast<T*>(a.q) + static_cast<size_t>(row) * a.q_stride + static_cast<size_t>(head) * a.d + chunk * 8) = out;
+    for (int h = 0; h < P8_HEADS; ++h) {
+        turn.apply(a, p8_row<T>(a, row, head + min(h, a.nq - 1 - head)), chunk, x[h]);
+        if (!written || head + h >= a.nq) continue;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) out.v[e] = from_float<T>(x[h][e]);
+        *reinterpret_cast<Piece*>(static_cast<T*>(a.q) + static_cast<size_t>(row) * a.q_stride + static_cast<size_t>(head + h) * a.d + chunk * 8) = out;
+    }
 }
 
 template <typename T, int LPR>
 static int launch_write(const P8Write& a, hipStream_t stream) {
     constexpr int WAVES = 4, ROWS = WAVES * PL_WAVE / LPR;
-    const int tile = 1;
-    const long groups = (a.slots != nullptr ? static_cast<long>(pl_ceil_div(a.n, tile)) * 2 * a.nkv : 0) + (static_cast<long>(a.n) * a.nq + ROWS - 1) / ROWS;
+    // A workgroup looks through `tile` rows for the first ones of runs.  One each while all of a step's may be first (decoding); with so many rows that most of them are inside a page 16, since
+    // a workgroup that finds nothing still costs its start (8,100 rows of prompts into 8 heads: TILE1 us with one, TILE16 with 16).
+    const int tile = static_cast<long>(a.n) * 2 * a.nkv <= 32768 ? 1 : 16;
+    const long groups = (a.slots != nullptr ? static_cast<long>(pl_ceil_div(a.n, tile)) * 2 * a.nkv : 0) + (static_cast<long>(a.n) * pl_ceil_div(a.nq, P8_HEADS) + ROWS - 1) / ROWS;
     PL_REQUIRE(groups < (1l << 31) && static_cast<long>(a.n) * a.nq < (1l << 31) - ROWS, "8-bit write: %d rows of %d heads are too many for a launch", a.n, a.nq + 2 * a.nkv);
-    write_8bit_kernel<T, LPR, WAVES><<<static_cast<unsigned>(groups), WAVES * PL_WAVE, 0, stream>>>(a, tile);
+    const bool pieces = a.rot == 0 || (a.rot % 16 == 0 && !a.neighbours && (reinterpret_cast<uintptr_t>(a.cos) | reinterpret_cast<uintptr_t>(a.sin)) % 16 == 0);
+    if (pieces) write_8bit_kernel<T, LPR, WAVES, true><<<static_cast<unsigned>(groups), WAVES * PL_WAVE, 0, stream>>>(a, tile);
+    else write_8bit_kernel<T, LPR, WAVES, false><<<static_cast<unsigned>(groups), WAVES * PL_WAVE, 0, stream>>>(a, tile);
     PL_CHECK_LAUNCH("write_8bit");
     return 0;
 }
