@@ -184,8 +184,7 @@ __global__ __launch_bounds__(A8_WAVES * PL_WAVE, PIECES * RB * DQ > 6 || (PIECES
     uint16_t* values = reinterpret_cast<uint16_t*>(lds);
     float* stats = reinterpret_cast<float*>(lds + VALUES);   // [waves][2][rows]
     int* slots = reinterpret_cast<int*>(stats + A8_WAVES * 2 * 16 * RB);
-    float* k_unit = reinterpret_cast<float*>(slots + a.chunk);
-    float* v_unit = k_unit + a.chunk;
+    uint16_t* units = reinterpret_cast<uint16_t*>(slots + a.chunk);          // (the two powers of a key, a byte each)
 
     const int tid = threadIdx.x, lane = tid % PL_WAVE, wave = tid / PL_WAVE;
     const int col = lane % 16, quarter = lane / 16;
@@ -204,8 +203,8 @@ __global__ __launch_bounds__(A8_WAVES * PL_WAVE, PIECES * RB * DQ > 6 || (PIECES
     for (int i = tid; i < a.chunk; i += A8_WAVES * PL_WAVE) {
         int page;
         slots[i] = a8_slot(a, seq, min(max(k_base + i, k_begin), k_end - 1), page);
-        k_unit[i] = a8_unit(a, a.k_scale, page, kvh);
-        v_unit[i] = a8_unit(a, a.v_scale, page, kvh);
+        const size_t at = static_cast<size_t>(page) * a.nkv + kvh;
+        units[i] = static_cast<uint16_t>(a.k_scale[at] | a.v_scale[at] << 8);
     }
 
     // The rows: what a lane reads of a key with its j-th load are the values 64 j + 16 quarter .. + 15, two operands
@@ -271,7 +270,7 @@ __global__ __launch_bounds__(A8_WAVES * PL_WAVE, PIECES * RB * DQ > 6 || (PIECES
 #pragma unroll
         for (int i = 0; i < LOADS; ++i) {
             const int at = i * PL_WAVE + lane, key = at / VP, piece = at % VP;
-            const float unit = v_unit[base + key];
+            const float unit = __uint_as_float(static_cast<uint32_t>(units[base + key] >> 8) << 23);
             a8_frag to[2];
 #pragma unroll
             for (int e = 0; e < 4; ++e) to[e / 2].half[e % 2] = a8_widen4(vraw[i][e], unit);
@@ -282,7 +281,7 @@ __global__ __launch_bounds__(A8_WAVES * PL_WAVE, PIECES * RB * DQ > 6 || (PIECES
         a8_f32x4 s[RB][2];
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-            const float unit = k_unit[base + 16 * half + col];
+            const float unit = __uint_as_float(static_cast<uint32_t>(units[base + 16 * half + col] & 0xff) << 23);
 #pragma unroll
             for (int b = 0; b < RB; ++b) s[b][half] = a8_f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -604,8 +603,9 @@ __global__ __launch_bounds__(A8_WAVES * PL_WAVE) void attention_8bit_merge_kerne
     const int first_row = rb * per, rows = min(per > 0 ? per : few, q_len * group - first_row);
     const int lo = pl_first_visible(start + first_row / group, a.window), hi = start + (first_row + rows - 1) / group + 1;
     const int all = a8_shares(lo, hi, a.chunk), shares = min(all, a.chunks);
-    const int threads = A8_WAVES * static_cast<int>(gridDim.y);
-    for (int r = threadIdx.x / PL_WAVE + A8_WAVES * blockIdx.y; r < rows; r += threads) {
+    const int waves = A8_WAVES * static_cast<int>(gridDim.y);
+    const int lanes = a.d <= 32 ? 8 : a.d <= 64 ? 16 : a.d <= 128 ? 32 : 64;        // of a share's row; the wave takes several shares at a time
+    for (int r = threadIdx.x / PL_WAVE + A8_WAVES * blockIdx.y; r < rows; r += waves) {
         const int row = first_row + r;
         const size_t out_row = static_cast<size_t>(a.q_start[seq] + row / group) * a.nq + kvh * group + row % group;
         const float* ml = a.part_ml + 2 * out_row * a.chunks;
@@ -615,45 +615,51 @@ __global__ __launch_bounds__(A8_WAVES * PL_WAVE) void attention_8bit_merge_kerne
         top = wave_max(top);
         const float base2 = top == -INFINITY ? 0.f : top;
         float total = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
+        const int at = 4 * (lane % lanes);
 #pragma unroll 4
-        for (int s = 0; s < shares; ++s) {
+        for (int s = lane / lanes; s < shares; s += PL_WAVE / lanes) {
             const float w = __builtin_amdgcn_exp2f(ml[2 * s] - base2);
             total += w * ml[2 * s + 1];
-            if (4 * lane < a.d) {
-                const a8_f32x4 y = *reinterpret_cast<const a8_f32x4*>(acc + static_cast<size_t>(s) * a.d + 4 * lane);
+            if (at < a.d) {
+                const a8_f32x4 y = *reinterpret_cast<const a8_f32x4*>(acc + static_cast<size_t>(s) * a.d + at);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) x[e] += w * y[e];
             }
         }
+        for (int off = lanes; off < PL_WAVE; off <<= 1) {
+            total += __shfl_xor(total, off, PL_WAVE);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] += __shfl_xor(x[e], off, PL_WAVE);
+        }
         if (all > shares) total = NAN;        // (a context longer than the caller said)
         const float inv = total != 0.f ? 1.f / total : 0.f;
-        if (4 * lane < a.d) {
+        if (lane < lanes && at < a.d) {
             struct __attribute__((aligned(4 * sizeof(T)))) Piece {
                 T v[4];
             } to;
 #pragma unroll
             for (int e = 0; e < 4; ++e) to.v[e] = from_float<T>(x[e] * inv);
-            *reinterpret_cast<Piece*>(static_cast<T*>(a.out) + out_row * a.d + 4 * lane) = to;
+            *reinterpret_cast<Piece*>(static_cast<T*>(a.out) + out_row * a.d + at) = to;
         }
     }
 }
 
 static int a8_lds(const void* kernel, size_t lds) {
-    if (lds <= 48 * 1024) return 0;
+    if (lds <= 64 * 1024) return 0;
     hipError_t e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds));
     PL_REQUIRE(e == hipSuccess, "8-bit attention: %zu bytes of LDS refused: %s", lds, hipGetErrorString(e));
     return 0;
 }
 
 template <int PIECES, int DQ, int RB>
-static int launch_few(const A8Args& a, hipStream_t stream) {
-    const size_t lds = static_cast<size_t>(A8_WAVES) * A8_KEYS * (64 * DQ + 16) * 2 + A8_WAVES * 2 * 16 * RB * 4 + static_cast<size_t>(a.chunk) * 12;
+static int launch_few(const A8Args& a, int rows, hipStream_t stream) {
+    const size_t lds = static_cast<size_t>(A8_WAVES) * A8_KEYS * (64 * DQ + 16) * 2 + A8_WAVES * 2 * 16 * RB * 4 + static_cast<size_t>(a.chunk) * 6;
     if (int e = a8_lds(reinterpret_cast<const void*>(&attention_8bit_few_kernel<PIECES, DQ, RB>), lds)) return e;
     const unsigned blocks = static_cast<unsigned>(a.S) * a.nkv;
     attention_8bit_few_kernel<PIECES, DQ, RB><<<dim3(blocks, a.chunks), A8_WAVES * PL_WAVE, lds, stream>>>(a);
     PL_CHECK_LAUNCH("attention_8bit_few");
     if (a.chunks > 1) {
-        attention_8bit_merge_kernel<typename A8Type<PIECES>::type><<<dim3(blocks, RB), A8_WAVES * PL_WAVE, 0, stream>>>(a, 16 * RB, 0);
+        attention_8bit_merge_kernel<typename A8Type<PIECES>::type><<<dim3(blocks, pl_ceil_div(rows, A8_WAVES)), A8_WAVES * PL_WAVE, 0, stream>>>(a, 16 * RB, 0);
         PL_CHECK_LAUNCH("attention_8bit_merge");
     }
     return 0;
@@ -662,12 +668,12 @@ static int launch_few(const A8Args& a, hipStream_t stream) {
 template <int PIECES, int DQ>
 static int launch_few(const A8Args& a, int rows, hipStream_t stream) {
     constexpr int MOST = A8Few<PIECES, DQ>::BLOCKS;
-    if (rows <= 16 || MOST == 1) return launch_few<PIECES, DQ, 1>(a, stream);
+    if (rows <= 16 || MOST == 1) return launch_few<PIECES, DQ, 1>(a, rows, stream);
     if constexpr (MOST >= 2)
-        if (rows <= 32 || MOST == 2) return launch_few<PIECES, DQ, 2>(a, stream);
+        if (rows <= 32 || MOST == 2) return launch_few<PIECES, DQ, 2>(a, rows, stream);
     if constexpr (MOST >= 4) {
-        if (rows <= 48) return launch_few<PIECES, DQ, 3>(a, stream);
-        return launch_few<PIECES, DQ, 4>(a, stream);
+        if (rows <= 48) return launch_few<PIECES, DQ, 3>(a, rows, stream);
+        return launch_few<PIECES, DQ, 4>(a, rows, stream);
     }
     return 0;
 }
@@ -735,15 +741,18 @@ extern "C" int pl_paged_attention_8bit(const void* q, int q_stride, void* out, c
     PL_REQUIRE(S >= 1 && n >= 1 && max_q_len >= 1 && min_q_len <= max_q_len && width >= 1 && block >= 1 && pool_rows >= block,
                "8-bit attention: %d requests, %d rows, %d to %d of one request, tables of %d pages of %d, %d rows", S, n, min_q_len, max_q_len, width, block, pool_rows);
     PL_REQUIRE(static_cast<long>(n) * nq < (1l << 31) && static_cast<long>(S) * nkv < (1l << 31), "8-bit attention: %d rows of %d heads, %d requests are too many for a launch", n, nq, S);
-    PL_REQUIRE(few_chunk >= A8_KEYS && few_chunk % A8_KEYS == 0 && few_chunk <= 4096 && few_chunks >= 1 && few_chunks < 65536 && (few_chunks == 1 || (part_acc && part_ml)),
+    PL_REQUIRE(few_chunk >= A8_KEYS && few_chunk % A8_KEYS == 0 && few_chunk <= 2048 && few_chunks >= 1 && few_chunks < 65536 && (few_chunks == 1 || (part_acc && part_ml)),
                "8-bit attention: %d shares of %d keys", few_chunks, few_chunk);
     PL_REQUIRE(many_chunk >= A8_TILE && many_chunk % A8_TILE == 0 && many_chunks >= 1 && many_chunks < 65536 && (many_chunks == 1 || (part_acc && part_ml)),
                "8-bit attention: %d shares of %d keys", many_chunks, many_chunk);
     A8Args a{q, q_stride, out, static_cast<const int*>(q_start), static_cast<const int*>(q_len), static_cast<const int*>(ctx_len), S, static_cast<const int*>(table), width, block, pool_rows,
              static_cast<const uint8_t*>(k_pool), static_cast<const uint8_t*>(v_pool), static_cast<const uint8_t*>(k_scale), static_cast<const uint8_t*>(v_scale),
              nq, nkv, d, scale * 1.4426950408889634f, window, n, few_chunk, few_chunks, static_cast<float*>(part_acc), static_cast<float*>(part_ml)};
-    const int few = pl_paged_attention_8bit_few(d, dtype);
     const long group = nq / nkv, longest = max_q_len * group;
+    // In a step of portions only what 16 rows hold goes to the kernel of few: those are the single tokens beside them, for which its smallest form is the fastest
+    // (15 single tokens at up to 4,600 keys beside a portion: 32 us with it, 91 with the form for 64 rows).
+    int few = pl_paged_attention_8bit_few(d, dtype);
+    if (longest > few) few = 16;
     const hipStream_t on = static_cast<hipStream_t>(stream);
     const bool f32 = dtype == PL_DTYPE_F32;
     if (longest > few) {

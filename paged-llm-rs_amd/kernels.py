@@ -2937,10 +2937,15 @@ class StepTables(NamedTuple):
     pages: torch.Tensor         # [1]
 
 
-def _here(t: torch.Tensor, what: str) -> None:
-    """Launches go to the current device's stream: a tensor of another device would be read from there."""
-    if t.device.index != torch.cuda.current_device():
-        raise TensorError(f"{what} is on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
+def _fits(t: torch.Tensor, what: str, dtype: torch.dtype, count: int, device: int, shape=None) -> int:
+    """The address of a tensor of ``count`` values that the launch can take: of this type, contiguous, on the current device (launches go to its stream, and a tensor of
+    another device would be read from there).  Asked for in few words, since a step of single tokens is as long as its launches take the host."""
+    if t.dtype is not dtype or t.get_device() != device or t.numel() != count or not t.is_contiguous() or (shape is not None and tuple(t.shape) != shape):
+        _need(t, what, shape, dtype)
+        if t.get_device() != device:
+            raise TensorError(f"{what} is on {t.device}, the current device is cuda:{device}")
+        raise TensorError(f"{what} has shape {tuple(t.shape)}, expected {count} values")
+    return t.data_ptr()
 
 
 def step_tables(q_len: torch.Tensor, ctx_len: torch.Tensor, block_table: torch.Tensor, block_size: int, free_pages: torch.Tensor | None, rows: int) -> StepTables:
@@ -2954,46 +2959,46 @@ def step_tables(q_len: torch.Tensor, ctx_len: torch.Tensor, block_table: torch.T
 
     Rows behind the last request's, up to ``rows``, and those of a request whose context is shorter than what it brings (the padding of a step) have position and slot -1;
     ``seq_of`` of rows behind the last is the last request."""
-    _need(q_len, "tokens of each request", None, torch.int32)
-    S = q_len.numel()
-    _need(ctx_len, "context length of each request", (S,), torch.int32)
-    _need(block_table, "block table", None, torch.int32)
-    _here(block_table, "block table")
+    S, device = q_len.numel(), torch.cuda.current_device()
     if q_len.dim() != 1 or not 1 <= S <= STEP_TABLES_MAX_SEQS:
         raise TensorError(f"tokens of each request have shape {tuple(q_len.shape)}, expected [1 to {STEP_TABLES_MAX_SEQS}]")
     if block_table.dim() != 2 or block_table.shape[0] != S or block_table.shape[1] < 1:
         raise TensorError(f"block table has shape {tuple(block_table.shape)}, expected [{S}, pages]")
-    if free_pages is not None:
-        _need(free_pages, "free pages", (free_pages.numel(),), torch.int32)
     if rows < 0 or block_size < 1:
         raise TensorError(f"{rows} rows of pages of {block_size} tokens")
-    made = StepTables(*torch.empty(3 * rows + S + 1, dtype=torch.int32, device=q_len.device).split([rows, rows, rows, S, 1]))
-    # (an empty list of free pages is a list: its address may be nothing, and any other stands for it)
-    free = 0 if free_pages is None else (free_pages.data_ptr() or block_table.data_ptr())
-    _check(library().pl_step_tables(q_len.data_ptr(), ctx_len.data_ptr(), S, block_table.data_ptr(), block_table.shape[1], block_size, free,
-                                    0 if free_pages is None else free_pages.numel(), rows, made.q_start.data_ptr(), made.positions.data_ptr(), made.seq_of.data_ptr(),
-                                    made.slots.data_ptr(), made.pages.data_ptr(), _stream()))
+    width = block_table.shape[1]
+    brings = _fits(q_len, "tokens of each request", torch.int32, S, device)
+    context = _fits(ctx_len, "context length of each request", torch.int32, S, device)
+    table = _fits(block_table, "block table", torch.int32, S * width, device)
+    free = count = 0
+    if free_pages is not None:
+        count = free_pages.numel()
+        # (an empty list of free pages is a list: its address may be nothing, and any other stands for it)
+        free = _fits(free_pages, "free pages", torch.int32, count, device) or table
+    room = q_len.new_empty(3 * rows + S + 1)
+    made = StepTables(*room.split_with_sizes([rows, rows, rows, S, 1]))
+    at = room.data_ptr()
+    _check(library().pl_step_tables(brings, context, S, table, width, block_size, free, count, rows, at + 12 * rows, at, at + 4 * rows, at + 8 * rows, at + 12 * rows + 4 * S,
+                                    _stream()))
     return made
 
 
-def _pages_8bit(k_pool, v_pool, k_scale, v_scale, block_size: int, nkv: int, d: int) -> int:
-    """The rows of the pools, once they are what the kernels take."""
+def _pages_8bit(k_pool, v_pool, k_scale, v_scale, block_size: int, nkv: int, d: int, device: int) -> tuple:
+    """(rows of the pools, the four addresses), once they are what the kernels take."""
     if not 16 <= d <= 256 or d % 16:
         raise TensorError(f"head size {d}: the 8-bit cache takes multiples of 16 up to 256")
-    _need(k_pool, "key pool", None, E4M3)
-    rows = k_pool.shape[0]
-    if block_size < 1 or nkv < 1 or k_pool.dim() != 2 or k_pool.shape[1] != nkv * d or rows % block_size or rows == 0:
-        raise TensorError(f"key pool has shape {tuple(k_pool.shape)}, expected [pages*{block_size}, {nkv * d}]")
+    shape = k_pool.shape
+    if block_size < 1 or nkv < 1 or len(shape) != 2 or shape[1] != nkv * d or shape[0] % block_size or shape[0] == 0:
+        raise TensorError(f"key pool has shape {tuple(shape)}, expected [pages*{block_size}, {nkv * d}]")
+    rows, width = shape
     if rows >= 2 ** 31:
         raise TensorError("a pool of 2^31 slots or more is not addressed by these kernels")
-    _need(v_pool, "value pool", k_pool.shape, E4M3)
-    pages = (rows // block_size, nkv)
-    _need(k_scale, "powers of the keys", pages, E8M0)
-    _need(v_scale, "powers of the values", pages, E8M0)
-    if not in_pieces(k_pool, v_pool):
+    scales = rows // block_size * nkv
+    keys, values = _fits(k_pool, "key pool", E4M3, rows * width, device), _fits(v_pool, "value pool", E4M3, rows * width, device, shape)
+    powers = (rows // block_size, nkv)
+    if (keys | values) % 16:
         raise TensorError("the pools of an 8-bit cache begin at whole 16 bytes")
-    _here(k_pool, "key pool")
-    return rows
+    return rows, keys, values, _fits(k_scale, "powers of the keys", E8M0, scales, device, powers), _fits(v_scale, "powers of the values", E8M0, scales, device, powers)
 
 
 def qk_norm_rope_kv_write_8bit(qkv: torch.Tensor, q: torch.Tensor | None, q_gain, k_gain, eps: float, cos, sin, rot: int, positions: torch.Tensor, slots: torch.Tensor,
@@ -3006,45 +3011,52 @@ def qk_norm_rope_kv_write_8bit(qkv: torch.Tensor, q: torch.Tensor | None, q_gain
 
     The rows that go into one page follow each other with slots that follow each other, as those of a request's tokens do, and no page is named twice; a slot below 0 (or past the
     pool) is written nowhere, and the queries of a row with a position below 0 are left as they were.  ``write_kv=False``: the queries alone."""
-    n = qkv.shape[0]
+    device = torch.cuda.current_device()
     code = _code(qkv, "fused q/k/v projection")
-    _need(qkv, "fused q/k/v projection", (n, (nq + 2 * nkv) * d))
-    rows = _pages_8bit(k_pool, v_pool, k_scale, v_scale, block_size, nkv, d)
-    _need(positions, "positions", (n,), torch.int32)
-    _need(slots, "slots", (n,), torch.int32)
-    if q is None:
-        q, stride = qkv, qkv.shape[1]
-    else:
-        _need(q, "queries", (n, nq * d), qkv.dtype)
-        stride = nq * d
-    gain_code = F32
+    rows, keys, values, key_powers, value_powers = _pages_8bit(k_pool, v_pool, k_scale, v_scale, block_size, nkv, d, device)
+    n, width = qkv.shape[0], (nq + 2 * nkv) * d
+    source = _fits(qkv, "fused q/k/v projection", qkv.dtype, n * width, device, (n, width))
+    queries, stride = source, width
+    if q is not None:
+        queries, stride = _fits(q, "queries", qkv.dtype, n * nq * d, device, (n, nq * d)), nq * d
     if (q_gain is None) != (k_gain is None):
         raise TensorError("queries and keys are normed both or neither")
+    gain_code = q_gains = k_gains = 0
     if q_gain is not None:
-        _need(q_gain, "query norm gain", (d,))
-        _need(k_gain, "key norm gain", (d,), q_gain.dtype)
         gain_code = _code(q_gain, "query norm gain")
+        q_gains, k_gains = _fits(q_gain, "query norm gain", q_gain.dtype, d, device), _fits(k_gain, "key norm gain", q_gain.dtype, d, device)
+    cosines = sines = angles = 0
     if rot:
-        _need(cos, "cosine table", None, torch.float32)
         if rot % 2 or not 0 < rot <= d or cos.dim() != 2 or cos.shape[1] != rot // 2 or cos.shape[0] < 1:
             raise TensorError(f"rotary tables have shape {tuple(cos.shape)}, expected [positions, {rot // 2}] for a rotation over {rot} values of a head of {d}")
-        _need(sin, "sine table", cos.shape, torch.float32)
-    if not in_pieces(qkv, q, q_gain, k_gain):
+        angles = cos.shape[0]
+        cosines, sines = _fits(cos, "cosine table", torch.float32, angles * (rot // 2), device), _fits(sin, "sine table", torch.float32, angles * (rot // 2), device, cos.shape)
+    if (source | queries | q_gains | k_gains) % 16:
         raise TensorError("rows and gains for an 8-bit cache begin at whole 16 bytes")
+    places = _fits(slots, "slots", torch.int32, n, device) if write_kv else 0
     _check(library().pl_qk_norm_rope_kv_write_8bit(
-        qkv.data_ptr(), q.data_ptr(), stride, _ptr(q_gain), _ptr(k_gain), gain_code, eps, cos.data_ptr() if rot else 0, sin.data_ptr() if rot else 0, rot,
-        cos.shape[0] if rot else 0, 1 if neighbours else 0, positions.data_ptr(), slots.data_ptr() if write_kv else 0, block_size, rows, k_pool.data_ptr(), v_pool.data_ptr(),
-        k_scale.data_ptr(), v_scale.data_ptr(), n, nq, nkv, d, code, _stream()))
+        source, queries, stride, q_gains, k_gains, gain_code, eps, cosines, sines, rot, angles, 1 if neighbours else 0, _fits(positions, "positions", torch.int32, n, device), places,
+        block_size, rows, keys, values, key_powers, value_powers, n, nq, nkv, d, code, _stream()))
 
 
 def shares_8bit(n: int, requests: int, max_ctx: int, nq: int, nkv: int, window: int = 0) -> tuple:
-    """(keys a share, shares) of the 8-bit attention's kernel of few rows, and the same of its kernel of many."""
-    few = many = 512
-    # (under a window a block of rows reaches over the window and its own tokens)
-    within = lambda chunk: min((max_ctx + chunk - 1) // chunk, (window + 256) // chunk + 2) if window > 0 else (max_ctx + chunk - 1) // chunk  # noqa: E731
-    if n * nq > 256 * 512:
-        many = (max_ctx + 63) // 64 * 64
-    return few, within(few), many, within(many)
+    """(keys a share, shares) of the 8-bit attention's kernel of few rows, and the same of its kernel of many.
+
+    Few rows: the longest shares, up to 2,048 keys, that still give the chip some 200 workgroups: every share costs a start of some 3 us and leaves a row of results to be put together.
+    Many rows: as many shares as make two workgroups a compute unit of the blocks of 256 rows, none of fewer than 512 keys, since a share writes and reads its rows' outputs in 32 bits."""
+    def of(chunk, reach):
+        # shares begin at whole ones of them, so what a block of rows sees under a mask may touch one more than it fills
+        every = (max_ctx + chunk - 1) // chunk
+        return chunk, min(every, (reach - 1) // chunk + 2) if window else every
+
+    reach = min(max_ctx, abs(window) + 64) if window else max_ctx
+    chunk = 2048
+    while chunk > 128 and requests * nkv * ((reach + chunk - 1) // chunk) < 200:
+        chunk //= 2
+    few = of(min(chunk, (max_ctx + 31) // 32 * 32), reach)
+    reach = min(max_ctx, abs(window) + 256) if window else max_ctx
+    shares = max(1, min(512 // ((n * (nq // nkv) + 255) // 256 * nkv), reach // 512))
+    return few + of((reach + 64 * shares - 1) // (64 * shares) * 64 if shares > 1 else (max_ctx + 63) // 64 * 64, reach)
 
 
 def paged_attention_8bit(q: torch.Tensor, q_row_stride: int, out: torch.Tensor, q_start: torch.Tensor, q_len: torch.Tensor, ctx_len: torch.Tensor, max_q_len: int,
@@ -3057,29 +3069,26 @@ def paged_attention_8bit(q: torch.Tensor, q_row_stride: int, out: torch.Tensor, 
 
     ``max_q_len``, ``min_q_len`` and ``max_ctx`` bound what the requests bring and their contexts (the launches are sized and chosen by them): rows whose keys reach past ``max_ctx`` come out as NaN, and
     rows past ``max_q_len`` of a request may be left out.  The caller answers for the pages of all keys that are seen; keys that no row of a request sees may hold anything."""
-    n = q.shape[0]
+    device = torch.cuda.current_device()
     code = _code(q, "query buffer")
-    _need(q, "query buffer")
-    if q.dim() != 2 or n < 1 or q.shape[1] != q_row_stride or q_row_stride < nq * d:
-        raise TensorError(f"query buffer has shape {tuple(q.shape)} for row stride {q_row_stride}")
     if nkv < 1 or nq < 1 or nq % nkv:
         raise TensorError(f"{nq} query heads over {nkv} key heads, which do not group evenly")
-    rows = _pages_8bit(k_pool, v_pool, k_scale, v_scale, block_size, nkv, d)
-    _need(out, "attention output", (n, nq * d), q.dtype)
-    _need(block_table, "block table", None, torch.int32)
-    S = block_table.shape[0]
-    if block_table.dim() != 2 or S < 1 or block_table.shape[1] < 1:
+    rows, keys, values, key_powers, value_powers = _pages_8bit(k_pool, v_pool, k_scale, v_scale, block_size, nkv, d, device)
+    n = q.shape[0]
+    if q.dim() != 2 or n < 1 or q.shape[1] != q_row_stride or q_row_stride < nq * d:
+        raise TensorError(f"query buffer has shape {tuple(q.shape)} for row stride {q_row_stride}")
+    S, width = block_table.shape if block_table.dim() == 2 else (0, 0)
+    if S < 1 or width < 1:
         raise TensorError(f"block table has shape {tuple(block_table.shape)}, expected [requests, pages]")
-    _need(q_start, "first row of each request", (S,), torch.int32)
-    _need(q_len, "tokens of each request", (S,), torch.int32)
-    _need(ctx_len, "context length of each request", (S,), torch.int32)
     if not 1 <= max_q_len <= n or not 0 <= min_q_len <= max_q_len or max_ctx < 1:
         raise TensorError(f"requests are said to bring {min_q_len} to {max_q_len} of the step's {n} tokens, contexts to be {max_ctx} at most")
     if not 0 < scale < math.inf:
         raise TensorError(f"scores scaled by {scale}, which has to be finite and above zero")
-    if q_row_stride % 8 or not in_pieces(q, out):
+    queries, results = _fits(q, "query buffer", q.dtype, n * q_row_stride, device), _fits(out, "attention output", q.dtype, n * nq * d, device, (n, nq * d))
+    if q_row_stride % 8 or (queries | results) % 16:
         raise TensorError("query rows and outputs for an 8-bit cache begin at whole 16 bytes")
-    few, few_shares, many, many_shares = shares_8bit(n, S, int(max_ctx), nq, nkv, int(window or 0))
+    window = int(window or 0)
+    few, few_shares, many, many_shares = shares_8bit(n, S, max_ctx, nq, nkv, window)
     chunks = max(few_shares, many_shares)
     acc = ml = 0
     if chunks > 1:
@@ -3087,7 +3096,7 @@ def paged_attention_8bit(q: torch.Tensor, q_row_stride: int, out: torch.Tensor, 
         acc = room.data_ptr()
         ml = acc + 4 * n * nq * chunks * d
     _check(library().pl_paged_attention_8bit(
-        q.data_ptr(), q_row_stride, out.data_ptr(), q_start.data_ptr(), q_len.data_ptr(), ctx_len.data_ptr(), S, n, max_q_len, min_q_len, block_table.data_ptr(),
-        block_table.shape[1], block_size, rows, k_pool.data_ptr(), v_pool.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), nq, nkv, d, scale, int(window or 0),
-        few, few_shares, many, many_shares, acc, ml, code, _stream()))
+        queries, q_row_stride, results, _fits(q_start, "first row of each request", torch.int32, S, device), _fits(q_len, "tokens of each request", torch.int32, S, device),
+        _fits(ctx_len, "context length of each request", torch.int32, S, device), S, n, max_q_len, min_q_len, _fits(block_table, "block table", torch.int32, S * width, device), width,
+        block_size, rows, keys, values, key_powers, value_powers, nq, nkv, d, scale, window, few, few_shares, many, many_shares, acc, ml, code, _stream()))
     return out
