@@ -43,7 +43,7 @@ struct A8Args {
     const int *q_start, *q_len, *ctx_len;
     int S;
     const int* table;
-    int width, block, pool_rows;
+    int width, block, shift, pages;      // (shift: of a page size that is a power of two, else -1)
     const uint8_t *k_pool, *v_pool, *k_scale, *v_scale;
     int nq, nkv, d;
     float scale;              // times log2(e)
@@ -140,14 +140,13 @@ __device__ __forceinline__ int a8_shares(int lo, int hi, int chunk) { return hi 
 
 // Where key `key` of request `seq` is in the pools, and its page.  (What the table does not say is read from page 0.)
 __device__ __forceinline__ int a8_slot(const A8Args& a, int seq, int key, int& page) {
-    const int index = key / a.block;
+    const int index = a.shift >= 0 ? key >> a.shift : key / a.block;
     page = index < a.width ? a.table[static_cast<size_t>(seq) * a.width + index] : 0;
-    page = page < 0 || page >= a.pool_rows / a.block ? 0 : page;
-    return page * a.block + key % a.block;
+    page = static_cast<unsigned>(page) < static_cast<unsigned>(a.pages) ? page : 0;
+    return page * a.block + key - index * a.block;
 }
-__device__ __forceinline__ float a8_unit(const A8Args& a, const uint8_t* scale, int page, int kvh) {
-    return __uint_as_float(static_cast<uint32_t>(scale[static_cast<size_t>(page) * a.nkv + kvh]) << 23);
-}
+// A page's power, a byte, as the number.
+__device__ __forceinline__ float a8_unit(uint32_t power) { return __uint_as_float(power << 23); }
 
 // Four neighbouring results of one row, as the caller's type.
 template <int PIECES>
@@ -209,15 +208,15 @@ __global__ __launch_bounds__(A8_WAVES * PL_WAVE, PIECES * RB * DQ > 6 || (PIECES
 
     // The rows: what a lane reads of a key with its j-th load are the values 64 j + 16 quarter .. + 15, two operands
     const int q_start = a.q_start[seq];
-    int position[RB], seen_from[RB], out_row[RB];
+    int seen_from[RB], seen[RB], out_row[RB];        // the keys of the share that a row sees: the first and how many
     a8_frag qf[RB][2 * DQ][PIECES];
 #pragma unroll
     for (int b = 0; b < RB; ++b) {
         const int row = 16 * b + col;
         const bool live = row < rows;
         const int token = live ? row / group : 0, head = kvh * group + (live ? row % group : 0);
-        position[b] = start + token;
-        seen_from[b] = pl_first_visible(position[b], a.window);
+        seen_from[b] = max(pl_first_visible(start + token, a.window), k_begin);
+        seen[b] = max(min(start + token + 1, k_end) - seen_from[b], 0);
         out_row[b] = live ? (q_start + token) * a.nq + head : -1;
 #pragma unroll
         for (int j = 0; j < 2 * DQ; ++j) {
@@ -270,7 +269,7 @@ __global__ __launch_bounds__(A8_WAVES * PL_WAVE, PIECES * RB * DQ > 6 || (PIECES
 #pragma unroll
         for (int i = 0; i < LOADS; ++i) {
             const int at = i * PL_WAVE + lane, key = at / VP, piece = at % VP;
-            const float unit = __uint_as_float(static_cast<uint32_t>(units[base + key] >> 8) << 23);
+            const float unit = a8_unit(units[base + key] >> 8);
             a8_frag to[2];
 #pragma unroll
             for (int e = 0; e < 4; ++e) to[e / 2].half[e % 2] = a8_widen4(vraw[i][e], unit);
@@ -281,7 +280,7 @@ __global__ __launch_bounds__(A8_WAVES * PL_WAVE, PIECES * RB * DQ > 6 || (PIECES
         a8_f32x4 s[RB][2];
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-            const float unit = __uint_as_float(static_cast<uint32_t>(units[base + 16 * half + col] & 0xff) << 23);
+            const float unit = a8_unit(units[base + 16 * half + col] & 0xff);
 #pragma unroll
             for (int b = 0; b < RB; ++b) s[b][half] = a8_f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -307,7 +306,7 @@ __global__ __launch_bounds__(A8_WAVES * PL_WAVE, PIECES * RB * DQ > 6 || (PIECES
                 x[e] = s[b][e / 4][e % 4] * a.scale;
                 if (!whole) {
                     const int key = k0 + 16 * (e / 4) + 4 * quarter + e % 4;
-                    x[e] = key >= k_begin && key < k_end && key <= position[b] && key >= seen_from[b] ? x[e] : -INFINITY;
+                    x[e] = static_cast<unsigned>(key - seen_from[b]) < static_cast<unsigned>(seen[b]) ? x[e] : -INFINITY;
                 }
                 top = fmaxf(top, x[e]);
             }
@@ -406,7 +405,7 @@ __global__ __launch_bounds__(A8_WAVES * PL_WAVE, PIECES * RB * DQ > 6 || (PIECES
 //   S^T = K . Q^T: v_mfma_f32_32x32x16_bf16; a lane has for row lane % 32 the keys 8 (i / 4) + 4 (lane / 32) + i % 4 of 32.  DT: the head is padded to 32 DT values.
 #define A8_TILE 64
 template <int PIECES, int DT, int NW>
-__global__ __launch_bounds__(NW * PL_WAVE, PIECES * DT >= 8 ? 1 : 2) void attention_8bit_many_kernel(A8Args a, int few) {
+__global__ __launch_bounds__(NW * PL_WAVE) __attribute__((amdgpu_waves_per_eu(PIECES * DT >= 8 ? 1 : 2, PIECES * DT >= 8 ? 1 : 2))) void attention_8bit_many_kernel(A8Args a, int few) {
     constexpr int DP = 32 * DT, KROW = DP + 8, VROW = DP + (DT % 2 == 0 ? 32 : 0), THREADS = NW * PL_WAVE;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     uint16_t* keys = reinterpret_cast<uint16_t*>(lds);                 // [2][64][KROW]
@@ -430,7 +429,8 @@ __global__ __launch_bounds__(NW * PL_WAVE, PIECES * DT >= 8 ? 1 : 2) void attent
     const int row = first_row + 32 * wave + col;
     const bool active = 32 * wave < rows, live = 32 * wave + col < rows;
     const int token = live ? row / group : (first_row + (active ? 32 * wave : 0)) / group, head = kvh * group + (live ? row % group : 0);
-    const int position = start + token, seen_from = pl_first_visible(position, a.window);
+    // the keys of the share that the lane's row sees: the first and how many
+    const int seen_from = max(pl_first_visible(start + token, a.window), k_begin), seen = max(min(start + token + 1, k_end) - seen_from, 0);
     const int first_pos = start + (first_row + (active ? 32 * wave : 0)) / group, last_pos = start + (first_row + min(32 * wave + 32, rows) - 1) / group;
     const int wave_from = pl_first_visible(first_pos, a.window), last_from = pl_first_visible(last_pos, a.window);
     a8_frag qf[2 * DT][PIECES];
@@ -440,25 +440,34 @@ __global__ __launch_bounds__(NW * PL_WAVE, PIECES * DT >= 8 ? 1 : 2) void attent
         a8_query8<PIECES>(a, static_cast<size_t>(q_start + token) * a.q_stride + static_cast<size_t>(head) * a.d + at, live && at < a.d, qf[j]);
     }
 
-    // A tile on its way: 16 bytes a lane and load, 2 DT lanes a key.
+    // Tiles on their way: 16 bytes a lane and load, 2 DT lanes a key.  The pages of a tile are asked for a round before its bytes, so that no round waits for one read behind another.
     constexpr int VP = 2 * DT, LOADS = (A8_TILE * VP + THREADS - 1) / THREADS;
     a8_u32x4 kraw[LOADS], vraw[LOADS];
-    float kun[LOADS], vun[LOADS];
-    auto fetch = [&](int k0) {
+    uint32_t kpow[LOADS], vpow[LOADS];      // (bytes as they come: made into a unit here they would be waited for here)
+    int pages[LOADS], offs[LOADS];
+    auto look = [&](int k0) {
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) {
+            const int at = i * THREADS + tid;
+            const int key = min(max(k0 + at / VP, k_begin), k_end - 1);      // (keys that no row sees are read at the nearest one's place)
+            const int index = a.shift >= 0 ? key >> a.shift : key / a.block;
+            offs[i] = key - index * a.block;
+            pages[i] = index < a.width ? a.table[static_cast<size_t>(seq) * a.width + index] : 0;
+        }
+    };
+    auto fetch = [&]() {
 #pragma unroll
         for (int i = 0; i < LOADS; ++i) {
             const int at = i * THREADS + tid, piece = at % VP;
+            const int page = static_cast<unsigned>(pages[i]) < static_cast<unsigned>(a.pages) ? pages[i] : 0;
+            const size_t from = (static_cast<size_t>(page * a.block + offs[i]) * a.nkv + kvh) * a.d + 16 * piece;
             kraw[i] = vraw[i] = a8_u32x4{0u, 0u, 0u, 0u};
-            kun[i] = vun[i] = 1.f;
             if (at < A8_TILE * VP && 16 * piece < a.d) {
-                int page;
-                const int slot = a8_slot(a, seq, min(max(k0 + at / VP, k_begin), k_end - 1), page);
-                const size_t from = (static_cast<size_t>(slot) * a.nkv + kvh) * a.d + 16 * piece;
                 kraw[i] = *reinterpret_cast<const a8_u32x4*>(a.k_pool + from);
                 vraw[i] = *reinterpret_cast<const a8_u32x4*>(a.v_pool + from);
-                kun[i] = a8_unit(a, a.k_scale, page, kvh);
-                vun[i] = a8_unit(a, a.v_scale, page, kvh);
             }
+            kpow[i] = a.k_scale[static_cast<size_t>(page) * a.nkv + kvh];
+            vpow[i] = a.v_scale[static_cast<size_t>(page) * a.nkv + kvh];
         }
     };
     auto put = [&](int buffer) {
@@ -468,12 +477,12 @@ __global__ __launch_bounds__(NW * PL_WAVE, PIECES * DT >= 8 ? 1 : 2) void attent
             if (at >= A8_TILE * VP) continue;
             a8_frag to[2];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) to[e / 2].half[e % 2] = a8_widen4(kraw[i][e], kun[i]);
+            for (int e = 0; e < 4; ++e) to[e / 2].half[e % 2] = a8_widen4(kraw[i][e], a8_unit(kpow[i]));
             uint16_t* k_to = keys + (buffer * A8_TILE + key) * KROW + 16 * piece;
             *reinterpret_cast<a8_u32x4*>(k_to) = to[0].raw;
             *reinterpret_cast<a8_u32x4*>(k_to + 8) = to[1].raw;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) to[e / 2].half[e % 2] = a8_widen4(vraw[i][e], vun[i]);
+            for (int e = 0; e < 4; ++e) to[e / 2].half[e % 2] = a8_widen4(vraw[i][e], a8_unit(vpow[i]));
             uint16_t* v_to = values + (buffer * A8_TILE + key) * VROW + 16 * piece;
             *reinterpret_cast<a8_u32x4*>(v_to) = to[0].raw;
             *reinterpret_cast<a8_u32x4*>(v_to + 8) = to[1].raw;
@@ -488,29 +497,44 @@ __global__ __launch_bounds__(NW * PL_WAVE, PIECES * DT >= 8 ? 1 : 2) void attent
     float m = -INFINITY, l = 0.f;
 
     const int k_first = k_begin / A8_TILE * A8_TILE;
-    fetch(k_first);
+    look(k_first);
+    fetch();
+    look(k_first + A8_TILE);
     put(0);
-    if (k_first + A8_TILE < k_end) fetch(k_first + A8_TILE);
+    fetch();
+    look(k_first + 2 * A8_TILE);
     __syncthreads();
     int buffer = 0;
     for (int k0 = k_first; k0 < k_end; k0 += A8_TILE, buffer ^= 1) {
         if (k0 + A8_TILE < k_end) put(buffer ^ 1);
-        if (k0 + 2 * A8_TILE < k_end) fetch(k0 + 2 * A8_TILE);
+        if (k0 + 2 * A8_TILE < k_end) {
+            fetch();
+            look(k0 + 3 * A8_TILE);
+        }
         if (active && k0 <= last_pos && k0 + A8_TILE > wave_from) {
             a8_f32x16 s[2];
             const uint16_t* k_from = keys + (buffer * A8_TILE + col) * KROW + 8 * half;
 #pragma unroll
-            for (int kb = 0; kb < 2; ++kb) {
+            for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) s[kb][i] = 0.f;
 #pragma unroll
-                for (int j = 0; j < 2 * DT; ++j) {
+            for (int j = 0; j < 2 * DT; ++j)
+#pragma unroll
+                for (int kb = 0; kb < 2; ++kb) {
                     a8_frag kf;
                     kf.raw = *reinterpret_cast<const a8_u32x4*>(k_from + 32 * kb * KROW + 16 * j);
 #pragma unroll
                     for (int p = PIECES - 1; p >= 0; --p) s[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf.vec, qf[j][p].vec, s[kb], 0, 0, 0);
                 }
+            // Six keys' operands are on their way while one is multiplied.
+            __builtin_amdgcn_sched_group_barrier(0x100, 6, 0);
+#pragma unroll
+            for (int j = 0; j < 4 * DT - 6; ++j) {
+                __builtin_amdgcn_sched_group_barrier(0x8, PIECES, 0);
+                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
             }
+            __builtin_amdgcn_sched_group_barrier(0x8, 6 * PIECES, 0);
             const bool whole = k0 >= k_begin && k0 >= last_from && k0 + A8_TILE <= k_end && k0 + A8_TILE - 1 <= first_pos;
             float top = -INFINITY;
 #pragma unroll
@@ -520,7 +544,7 @@ __global__ __launch_bounds__(NW * PL_WAVE, PIECES * DT >= 8 ? 1 : 2) void attent
                     float x = s[kb][i];
                     if (!whole) {
                         const int key = k0 + 32 * kb + 8 * (i / 4) + 4 * half + i % 4;
-                        x = key >= k_begin && key < k_end && key <= position && key >= seen_from ? x : -INFINITY;
+                        x = static_cast<unsigned>(key - seen_from) < static_cast<unsigned>(seen) ? x : -INFINITY;
                     }
                     s[kb][i] = x;
                     top = fmaxf(top, x);
@@ -540,8 +564,18 @@ __global__ __launch_bounds__(NW * PL_WAVE, PIECES * DT >= 8 ? 1 : 2) void attent
             const float from = m == -INFINITY ? 0.f : m;
             float sum = 0.f;
             const uint16_t* v_from = values + (buffer * A8_TILE + 4 * half + lane % 16 / 4) * VROW + 16 * (lane / 16 % 2) + 4 * (lane % 4);
+            a8_frag vf[2][DT];
+            auto read_values = [&](int g) {
+#pragma unroll
+                for (int t = 0; t < DT; ++t) {
+                    vf[g % 2][t].half[0] = a8_read_transposed(v_from + 16 * g * VROW + 32 * t);
+                    vf[g % 2][t].half[1] = a8_read_transposed(v_from + (16 * g + 8) * VROW + 32 * t);
+                }
+            };
+            read_values(0);
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
+                if (g < 3) read_values(g + 1);
                 float x[8];
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
@@ -551,13 +585,9 @@ __global__ __launch_bounds__(NW * PL_WAVE, PIECES * DT >= 8 ? 1 : 2) void attent
                 a8_frag pf[PIECES];
                 a8_split<PIECES>(x, pf);
 #pragma unroll
-                for (int t = 0; t < DT; ++t) {
-                    a8_frag vf;
-                    vf.half[0] = a8_read_transposed(v_from + 16 * g * VROW + 32 * t);
-                    vf.half[1] = a8_read_transposed(v_from + (16 * g + 8) * VROW + 32 * t);
+                for (int t = 0; t < DT; ++t)
 #pragma unroll
-                    for (int p = PIECES - 1; p >= 0; --p) acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf.vec, pf[p].vec, acc[t], 0, 0, 0);
-                }
+                    for (int p = PIECES - 1; p >= 0; --p) acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[g % 2][t].vec, pf[p].vec, acc[t], 0, 0, 0);
             }
             l += sum;
         }
@@ -704,7 +734,7 @@ static int launch_many(const A8Args& a, int few, long blocks, hipStream_t stream
 
 template <int PIECES, int DT>
 static int launch_many(const A8Args& a, int few, int max_q_len, hipStream_t stream) {
-    constexpr int NW = PIECES * DT >= 8 ? 4 : 8;
+    constexpr int NW = 4;
     const int group = a.nq / a.nkv;
     // blocks of rows: one a request for what is left over, and the whole ones
     const long most = static_cast<long>(a.S) * ((static_cast<long>(max_q_len) * group + 32 * NW - 1) / (32 * NW)), all = a.S + static_cast<long>(a.n) * group / (32 * NW);
@@ -745,7 +775,7 @@ extern "C" int pl_paged_attention_8bit(const void* q, int q_stride, void* out, c
                "8-bit attention: %d shares of %d keys", few_chunks, few_chunk);
     PL_REQUIRE(many_chunk >= A8_TILE && many_chunk % A8_TILE == 0 && many_chunks >= 1 && many_chunks < 65536 && (many_chunks == 1 || (part_acc && part_ml)),
                "8-bit attention: %d shares of %d keys", many_chunks, many_chunk);
-    A8Args a{q, q_stride, out, static_cast<const int*>(q_start), static_cast<const int*>(q_len), static_cast<const int*>(ctx_len), S, static_cast<const int*>(table), width, block, pool_rows,
+    A8Args a{q, q_stride, out, static_cast<const int*>(q_start), static_cast<const int*>(q_len), static_cast<const int*>(ctx_len), S, static_cast<const int*>(table), width, block, (block & (block - 1)) == 0 ? __builtin_ctz(block) : -1, pool_rows / block,
              static_cast<const uint8_t*>(k_pool), static_cast<const uint8_t*>(v_pool), static_cast<const uint8_t*>(k_scale), static_cast<const uint8_t*>(v_scale),
              nq, nkv, d, scale * 1.4426950408889634f, window, n, few_chunk, few_chunks, static_cast<float*>(part_acc), static_cast<float*>(part_ml)};
     const long group = nq / nkv, longest = max_q_len * group;
