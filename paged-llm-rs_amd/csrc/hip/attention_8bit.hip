@@ -43,7 +43,9 @@ struct A8Args {
     const int *q_start, *q_len, *ctx_len;
     int S;
     const int* table;
-    int width, block, shift, pages;      // (shift: of a page size that is a power of two, else -1)
+    int width, block;
+    uint32_t magic;           // of the division by `block` (a8_page_index)
+    int shift, pages;
     const uint8_t *k_pool, *v_pool, *k_scale, *v_scale;
     int nq, nkv, d;
     float scale;              // times log2(e)
@@ -138,10 +140,12 @@ __device__ __forceinline__ bool a8_find(const A8Args& a, int slot, int group, in
 // The keys [lo, hi) that a block of rows sees, cut into shares of `chunk` that begin at whole chunks: how many there are.
 __device__ __forceinline__ int a8_shares(int lo, int hi, int chunk) { return hi > lo ? (hi - 1) / chunk - lo / chunk + 1 : 0; }
 
-// Where key `key` of request `seq` is in the pools, and its page.  (What the table does not say is read from page 0.)
+// Which of its request's pages a key is in: a division by the page size, as a product with ceil(2^shift / block), shift = 31 + ceil(log2(block)), exact below 2^31.
+__device__ __forceinline__ int a8_page_index(const A8Args& a, int key) { return static_cast<int>(static_cast<uint64_t>(static_cast<uint32_t>(key)) * a.magic >> a.shift); }
+// Where key `key` of request `seq` is in the pools, and its page.  (What the table says nothing sensible of is read from page 0.)
 __device__ __forceinline__ int a8_slot(const A8Args& a, int seq, int key, int& page) {
-    const int index = a.shift >= 0 ? key >> a.shift : key / a.block;
-    page = index < a.width ? a.table[static_cast<size_t>(seq) * a.width + index] : 0;
+    const int index = a8_page_index(a, key);
+    page = a.table[static_cast<size_t>(seq) * a.width + min(index, a.width - 1)];
     page = static_cast<unsigned>(page) < static_cast<unsigned>(a.pages) ? page : 0;
     return page * a.block + key - index * a.block;
 }
@@ -400,18 +404,33 @@ __global__ __launch_bounds__(A8_WAVES * PL_WAVE, PIECES * RB * DQ > 6 || (PIECES
 }
 
 // ---- many rows: every wave has rows of its own -----------------------------------------------------------------------------
-// A workgroup takes NW blocks of 32 rows of one request and key head and one share of the keys, a block a wave.  Tiles of 64 keys come into LDS as bfloat16, two lengths of them: while one is worked on, the bytes of the
-// next (which came into registers a tile earlier) are widened into the other, so what an e4m3 value costs to widen is paid once for all the rows, and a round has one barrier.
+// A workgroup takes NW blocks of 32 rows of one request and key head and one share of the keys, a block a wave.  Tiles of 32 KB keys come into LDS as bfloat16, so what an e4m3 value costs to widen is
+// paid once for all the rows.
 //   S^T = K . Q^T: v_mfma_f32_32x32x16_bf16; a lane has for row lane % 32 the keys 8 (i / 4) + 4 (lane / 32) + i % 4 of 32.  DT: the head is padded to 32 DT values.
-#define A8_TILE 64
-template <int PIECES, int DT, int NW>
-__global__ __launch_bounds__(NW * PL_WAVE) __attribute__((amdgpu_waves_per_eu(PIECES * DT >= 8 ? 1 : 2, PIECES * DT >= 8 ? 1 : 2))) void attention_8bit_many_kernel(A8Args a, int few) {
-    constexpr int DP = 32 * DT, KROW = DP + 8, VROW = DP + (DT % 2 == 0 ? 32 : 0), THREADS = NW * PL_WAVE;
-    extern __shared__ __attribute__((aligned(16))) char lds[];
-    uint16_t* keys = reinterpret_cast<uint16_t*>(lds);                 // [2][64][KROW]
-    uint16_t* values = keys + 2 * A8_TILE * KROW;                      // [2][64][VROW]
+// What bounds it is the weights: an exponential takes a wave four times as long as another vector instruction, and together they take as long as the products.  So the scores of the next tile are multiplied while
+// the weights of this one are made, and the next maximum is found while this tile's weights meet its values: both pipes work in one wave, whatever the other waves of the unit do.
+// For that the keys in LDS are a tile ahead of the values (two lengths of keys, three of values), their bytes another tile ahead in registers, and their pages one more.  A round has one barrier.
+template <int DT>
+struct A8Many {
+    static constexpr int KB = DT == 8 ? 1 : 2;          // (what 160 KB of LDS hold)
+    static constexpr int KROW = 32 * DT + 8, VROW = 32 * DT + (DT % 2 == 0 ? 32 : 0);
+    static constexpr size_t LDS = static_cast<size_t>(32 * KB) * (2 * KROW + 3 * VROW) * 2;
+};
 
-    const int tid = threadIdx.x, lane = tid % PL_WAVE, wave = tid / PL_WAVE;
+// The maximum of a lane's number and that of lane ^ 32.
+__device__ __forceinline__ float a8_max_half(float v) {
+    const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1]));
+}
+
+template <int PIECES, int DT, int NW>
+__global__ __launch_bounds__(NW * PL_WAVE) __attribute__((amdgpu_waves_per_eu(NW == 8 ? 2 : 1, NW == 8 ? 2 : 1))) void attention_8bit_many_kernel(A8Args a, int few) {
+    constexpr int KB = A8Many<DT>::KB, TILE = 32 * KB, KROW = A8Many<DT>::KROW, VROW = A8Many<DT>::VROW, THREADS = NW * PL_WAVE;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    uint16_t* keys = reinterpret_cast<uint16_t*>(lds);                 // [2][TILE][KROW]
+    uint16_t* values = keys + 2 * TILE * KROW;                         // [3][TILE][VROW]
+
+    const int tid = threadIdx.x, lane = tid % PL_WAVE, wave = __builtin_amdgcn_readfirstlane(tid / PL_WAVE);
     const int col = lane % 32, half = lane / 32;
     const int group = a.nq / a.nkv;
     const int kvh = blockIdx.x % a.nkv;
@@ -441,49 +460,48 @@ __global__ __launch_bounds__(NW * PL_WAVE) __attribute__((amdgpu_waves_per_eu(PI
     }
 
     // Tiles on their way: 16 bytes a lane and load, 2 DT lanes a key.  The pages of a tile are asked for a round before its bytes, so that no round waits for one read behind another.
-    constexpr int VP = 2 * DT, LOADS = (A8_TILE * VP + THREADS - 1) / THREADS;
+    constexpr int VP = 2 * DT, LOADS = (TILE * VP + THREADS - 1) / THREADS;
     a8_u32x4 kraw[LOADS], vraw[LOADS];
     uint32_t kpow[LOADS], vpow[LOADS];      // (bytes as they come: made into a unit here they would be waited for here)
     int pages[LOADS], offs[LOADS];
+    // (No load stands under a condition: what comes behind one is waited for where the paths meet.  A lane without a piece of a head reads the last one, whose products the queries' zeros take out.)
+    const int last_piece = a.d / 16 - 1;
     auto look = [&](int k0) {
 #pragma unroll
         for (int i = 0; i < LOADS; ++i) {
             const int at = i * THREADS + tid;
             const int key = min(max(k0 + at / VP, k_begin), k_end - 1);      // (keys that no row sees are read at the nearest one's place)
-            const int index = a.shift >= 0 ? key >> a.shift : key / a.block;
+            const int index = a8_page_index(a, key);
             offs[i] = key - index * a.block;
-            pages[i] = index < a.width ? a.table[static_cast<size_t>(seq) * a.width + index] : 0;
+            pages[i] = a.table[static_cast<size_t>(seq) * a.width + min(index, a.width - 1)];
         }
     };
     auto fetch = [&]() {
 #pragma unroll
         for (int i = 0; i < LOADS; ++i) {
-            const int at = i * THREADS + tid, piece = at % VP;
+            const int piece = min((i * THREADS + tid) % VP, last_piece);
             const int page = static_cast<unsigned>(pages[i]) < static_cast<unsigned>(a.pages) ? pages[i] : 0;
             const size_t from = (static_cast<size_t>(page * a.block + offs[i]) * a.nkv + kvh) * a.d + 16 * piece;
-            kraw[i] = vraw[i] = a8_u32x4{0u, 0u, 0u, 0u};
-            if (at < A8_TILE * VP && 16 * piece < a.d) {
-                kraw[i] = *reinterpret_cast<const a8_u32x4*>(a.k_pool + from);
-                vraw[i] = *reinterpret_cast<const a8_u32x4*>(a.v_pool + from);
-            }
+            kraw[i] = *reinterpret_cast<const a8_u32x4*>(a.k_pool + from);
+            vraw[i] = *reinterpret_cast<const a8_u32x4*>(a.v_pool + from);
             kpow[i] = a.k_scale[static_cast<size_t>(page) * a.nkv + kvh];
             vpow[i] = a.v_scale[static_cast<size_t>(page) * a.nkv + kvh];
         }
     };
-    auto put = [&](int buffer) {
+    auto put = [&](int k_buffer, int v_buffer) {
 #pragma unroll
         for (int i = 0; i < LOADS; ++i) {
             const int at = i * THREADS + tid, key = at / VP, piece = at % VP;
-            if (at >= A8_TILE * VP) continue;
+            if (TILE * VP % THREADS != 0 && at >= TILE * VP) continue;
             a8_frag to[2];
 #pragma unroll
             for (int e = 0; e < 4; ++e) to[e / 2].half[e % 2] = a8_widen4(kraw[i][e], a8_unit(kpow[i]));
-            uint16_t* k_to = keys + (buffer * A8_TILE + key) * KROW + 16 * piece;
+            uint16_t* k_to = keys + (k_buffer * TILE + key) * KROW + 16 * piece;
             *reinterpret_cast<a8_u32x4*>(k_to) = to[0].raw;
             *reinterpret_cast<a8_u32x4*>(k_to + 8) = to[1].raw;
 #pragma unroll
             for (int e = 0; e < 4; ++e) to[e / 2].half[e % 2] = a8_widen4(vraw[i][e], a8_unit(vpow[i]));
-            uint16_t* v_to = values + (buffer * A8_TILE + key) * VROW + 16 * piece;
+            uint16_t* v_to = values + (v_buffer * TILE + key) * VROW + 16 * piece;
             *reinterpret_cast<a8_u32x4*>(v_to) = to[0].raw;
             *reinterpret_cast<a8_u32x4*>(v_to + 8) = to[1].raw;
         }
@@ -494,62 +512,48 @@ __global__ __launch_bounds__(NW * PL_WAVE) __attribute__((amdgpu_waves_per_eu(PI
     for (int t = 0; t < DT; ++t)
 #pragma unroll
         for (int i = 0; i < 16; ++i) acc[t][i] = 0.f;
-    float m = -INFINITY, l = 0.f;
+    float m = -INFINITY, l = 0.f, top = -INFINITY;
 
-    const int k_first = k_begin / A8_TILE * A8_TILE;
-    look(k_first);
-    fetch();
-    look(k_first + A8_TILE);
-    put(0);
-    fetch();
-    look(k_first + 2 * A8_TILE);
-    __syncthreads();
-    int buffer = 0;
-    for (int k0 = k_first; k0 < k_end; k0 += A8_TILE, buffer ^= 1) {
-        if (k0 + A8_TILE < k_end) put(buffer ^ 1);
-        if (k0 + 2 * A8_TILE < k_end) {
-            fetch();
-            look(k0 + 3 * A8_TILE);
-        }
-        if (active && k0 <= last_pos && k0 + A8_TILE > wave_from) {
-            a8_f32x16 s[2];
-            const uint16_t* k_from = keys + (buffer * A8_TILE + col) * KROW + 8 * half;
+    const int k_first = k_begin / TILE * TILE, tiles = pl_ceil_div(k_end - k_first, TILE);
+    // The wave's rows see something of the tile at k0, or all of it.
+    auto sees = [&](int k0) { return active && k0 <= last_pos && k0 + TILE > wave_from; };
+    auto whole = [&](int k0) { return k0 >= k_begin && k0 >= last_from && k0 + TILE <= k_end && k0 + TILE - 1 <= first_pos; };
+    auto scores = [&](a8_f32x16 (&s)[KB], int buffer) {
+        const uint16_t* from = keys + (buffer * TILE + col) * KROW + 8 * half;
 #pragma unroll
-            for (int kb = 0; kb < 2; ++kb)
+        for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) s[kb][i] = 0.f;
+            for (int i = 0; i < 16; ++i) s[kb][i] = 0.f;
 #pragma unroll
-            for (int j = 0; j < 2 * DT; ++j)
+        for (int j = 0; j < 2 * DT; ++j)
 #pragma unroll
-                for (int kb = 0; kb < 2; ++kb) {
-                    a8_frag kf;
-                    kf.raw = *reinterpret_cast<const a8_u32x4*>(k_from + 32 * kb * KROW + 16 * j);
+            for (int kb = 0; kb < KB; ++kb) {
+                a8_frag kf;
+                kf.raw = *reinterpret_cast<const a8_u32x4*>(from + 32 * kb * KROW + 16 * j);
 #pragma unroll
-                    for (int p = PIECES - 1; p >= 0; --p) s[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf.vec, qf[j][p].vec, s[kb], 0, 0, 0);
-                }
-            // Six keys' operands are on their way while one is multiplied.
-            __builtin_amdgcn_sched_group_barrier(0x100, 6, 0);
-#pragma unroll
-            for (int j = 0; j < 4 * DT - 6; ++j) {
-                __builtin_amdgcn_sched_group_barrier(0x8, PIECES, 0);
-                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                for (int p = PIECES - 1; p >= 0; --p) s[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf.vec, qf[j][p].vec, s[kb], 0, 0, 0);
             }
-            __builtin_amdgcn_sched_group_barrier(0x8, 6 * PIECES, 0);
-            const bool whole = k0 >= k_begin && k0 >= last_from && k0 + A8_TILE <= k_end && k0 + A8_TILE - 1 <= first_pos;
-            float top = -INFINITY;
+    };
+    auto mask = [&](a8_f32x16 (&s)[KB], int k0) {
 #pragma unroll
-            for (int kb = 0; kb < 2; ++kb)
+        for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    float x = s[kb][i];
-                    if (!whole) {
-                        const int key = k0 + 32 * kb + 8 * (i / 4) + 4 * half + i % 4;
-                        x = static_cast<unsigned>(key - seen_from) < static_cast<unsigned>(seen) ? x : -INFINITY;
-                    }
-                    s[kb][i] = x;
-                    top = fmaxf(top, x);
-                }
-            top = fmaxf(top, __shfl_xor(top, 32, PL_WAVE)) * a.scale;
+            for (int i = 0; i < 16; ++i) {
+                const int key = k0 + 32 * kb + 8 * (i / 4) + 4 * half + i % 4;
+                s[kb][i] = static_cast<unsigned>(key - seen_from) < static_cast<unsigned>(seen) ? s[kb][i] : -INFINITY;
+            }
+    };
+    auto largest = [&](const a8_f32x16 (&s)[KB]) {
+        float most = s[0][0];
+#pragma unroll
+        for (int i = 1; i < 16 * KB; ++i) most = fmaxf(most, s[i / 16][i % 16]);
+        return a8_max_half(most) * a.scale;
+    };
+    // Round t: this tile's weights and values, the next one's scores, the one's bytes behind that.
+    int v_now = 0;
+    auto round = [&](a8_f32x16 (&s)[KB], a8_f32x16 (&next)[KB], int t) {
+        const int k0 = k_first + t * TILE, v_put = v_now == 0 ? 2 : v_now - 1;
+        if (sees(k0)) {
             // Weights are taken relative to a maximum that is at most 2^8 off: sums and outputs are scaled anew only where a row's maximum has grown by more.
             if (__any(top > m + 8.f)) {
                 const float grown = fmaxf(m, top);
@@ -562,36 +566,86 @@ __global__ __launch_bounds__(NW * PL_WAVE) __attribute__((amdgpu_waves_per_eu(PI
                     for (int i = 0; i < 16; ++i) acc[t][i] *= alpha;
             }
             const float from = m == -INFINITY ? 0.f : m;
+            scores(next, (t + 1) % 2);
+            a8_frag pf[2 * KB][PIECES];
             float sum = 0.f;
-            const uint16_t* v_from = values + (buffer * A8_TILE + 4 * half + lane % 16 / 4) * VROW + 16 * (lane / 16 % 2) + 4 * (lane % 4);
-            a8_frag vf[2][DT];
-            auto read_values = [&](int g) {
 #pragma unroll
-                for (int t = 0; t < DT; ++t) {
-                    vf[g % 2][t].half[0] = a8_read_transposed(v_from + 16 * g * VROW + 32 * t);
-                    vf[g % 2][t].half[1] = a8_read_transposed(v_from + (16 * g + 8) * VROW + 32 * t);
-                }
-            };
-            read_values(0);
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                if (g < 3) read_values(g + 1);
+            for (int g = 0; g < 2 * KB; ++g) {
                 float x[8];
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     x[e] = __builtin_amdgcn_exp2f(fmaf(s[g / 2][8 * (g % 2) + e], a.scale, -from));
                     sum += x[e];
                 }
-                a8_frag pf[PIECES];
-                a8_split<PIECES>(x, pf);
-#pragma unroll
-                for (int t = 0; t < DT; ++t)
-#pragma unroll
-                    for (int p = PIECES - 1; p >= 0; --p) acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[g % 2][t].vec, pf[p].vec, acc[t], 0, 0, 0);
+                a8_split<PIECES>(x, pf[g]);
             }
             l += sum;
+            // (Both orders of work are put side by side here: between two products on the matrix cores, their operands' read and a share of the weights.  Made by the
+            // compiler, the weights follow the products, and even go behind the branch below.)
+            __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+            for (int i = 0; i < 2 * DT * KB; ++i) {
+                __builtin_amdgcn_sched_group_barrier(0x8, PIECES, 0);
+                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x402, PIECES == 1 ? (28 + 2 * DT - 1) / (2 * DT) : (56 + 2 * DT - 1) / (2 * DT), 0);
+            }
+#pragma unroll
+            for (int g = 0; g < 2 * KB; ++g)
+#pragma unroll
+                for (int p = 0; p < PIECES; ++p) asm volatile("" : "+v"(pf[g][p].raw));
+            if (!whole(k0 + TILE)) mask(next, k0 + TILE);
+            top = largest(next);
+            const uint16_t* v_from = values + (v_now * TILE + 4 * half + lane % 16 / 4) * VROW + 16 * (lane / 16 % 2) + 4 * (lane % 4);
+#pragma unroll
+            for (int g = 0; g < 2 * KB; ++g)
+#pragma unroll
+                for (int t = 0; t < DT; ++t) {
+                    a8_frag vf;
+                    vf.half[0] = a8_read_transposed(v_from + 16 * g * VROW + 32 * t);
+                    vf.half[1] = a8_read_transposed(v_from + (16 * g + 8) * VROW + 32 * t);
+#pragma unroll
+                    for (int p = PIECES - 1; p >= 0; --p) acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf.vec, pf[g][p].vec, acc[t], 0, 0, 0);
+                }
+            __builtin_amdgcn_sched_group_barrier(0x100, 6, 0);
+#pragma unroll
+            for (int i = 0; i < 2 * DT * KB; ++i) {
+                __builtin_amdgcn_sched_group_barrier(0x8, PIECES, 0);
+                __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+                __builtin_amdgcn_sched_group_barrier(0x2, 3, 0);
+            }
+        } else if (sees(k0 + TILE)) {
+            scores(next, (t + 1) % 2);
+            mask(next, k0 + TILE);
+            top = largest(next);
         }
+        put(t % 2, v_put);
+        fetch();
+        look(k0 + 4 * TILE);
+        v_now = v_now == 2 ? 0 : v_now + 1;
         __syncthreads();
+    };
+
+    // (beyond the last tile the nearest key is read once more: no round goes by whether there is a next one)
+    look(k_first);
+    fetch();
+    look(k_first + TILE);
+    put(0, 0);
+    fetch();
+    look(k_first + 2 * TILE);
+    put(1, 1);
+    fetch();
+    look(k_first + 3 * TILE);
+    __syncthreads();
+    a8_f32x16 s[2][KB];
+    if (sees(k_first)) {
+        scores(s[0], 0);
+        mask(s[0], k_first);
+        top = largest(s[0]);
+    }
+    __syncthreads();
+    for (int t = 0; t < tiles; t += 2) {
+        round(s[0], s[1], t);
+        if (t + 1 < tiles) round(s[1], s[0], t + 1);
     }
     l += __shfl_xor(l, 32, PL_WAVE);
     if (!live) return;
@@ -720,7 +774,7 @@ static int launch_few(const A8Args& a, int rows, hipStream_t stream) {
 
 template <int PIECES, int DT, int NW>
 static int launch_many(const A8Args& a, int few, long blocks, hipStream_t stream) {
-    const size_t lds = 2 * static_cast<size_t>(A8_TILE) * (32 * DT + 8 + 32 * DT + (DT % 2 == 0 ? 32 : 0)) * 2;
+    const size_t lds = A8Many<DT>::LDS;
     if (int e = a8_lds(reinterpret_cast<const void*>(&attention_8bit_many_kernel<PIECES, DT, NW>), lds)) return e;
     PL_REQUIRE(blocks * a.nkv < (1l << 31), "8-bit attention: %ld blocks of rows are too many for a launch", blocks);
     attention_8bit_many_kernel<PIECES, DT, NW><<<dim3(static_cast<unsigned>(blocks * a.nkv), a.chunks), NW * PL_WAVE, lds, stream>>>(a, few);
@@ -734,7 +788,7 @@ static int launch_many(const A8Args& a, int few, long blocks, hipStream_t stream
 
 template <int PIECES, int DT>
 static int launch_many(const A8Args& a, int few, int max_q_len, hipStream_t stream) {
-    constexpr int NW = 4;
+    constexpr int NW = PIECES * DT >= 6 ? 4 : 8;
     const int group = a.nq / a.nkv;
     // blocks of rows: one a request for what is left over, and the whole ones
     const long most = static_cast<long>(a.S) * ((static_cast<long>(max_q_len) * group + 32 * NW - 1) / (32 * NW)), all = a.S + static_cast<long>(a.n) * group / (32 * NW);
@@ -773,9 +827,11 @@ extern "C" int pl_paged_attention_8bit(const void* q, int q_stride, void* out, c
     PL_REQUIRE(static_cast<long>(n) * nq < (1l << 31) && static_cast<long>(S) * nkv < (1l << 31), "8-bit attention: %d rows of %d heads, %d requests are too many for a launch", n, nq, S);
     PL_REQUIRE(few_chunk >= A8_KEYS && few_chunk % A8_KEYS == 0 && few_chunk <= 2048 && few_chunks >= 1 && few_chunks < 65536 && (few_chunks == 1 || (part_acc && part_ml)),
                "8-bit attention: %d shares of %d keys", few_chunks, few_chunk);
-    PL_REQUIRE(many_chunk >= A8_TILE && many_chunk % A8_TILE == 0 && many_chunks >= 1 && many_chunks < 65536 && (many_chunks == 1 || (part_acc && part_ml)),
+    PL_REQUIRE(many_chunk >= 64 && many_chunk % 64 == 0 && many_chunks >= 1 && many_chunks < 65536 && (many_chunks == 1 || (part_acc && part_ml)),
                "8-bit attention: %d shares of %d keys", many_chunks, many_chunk);
-    A8Args a{q, q_stride, out, static_cast<const int*>(q_start), static_cast<const int*>(q_len), static_cast<const int*>(ctx_len), S, static_cast<const int*>(table), width, block, (block & (block - 1)) == 0 ? __builtin_ctz(block) : -1, pool_rows / block,
+    const int shift = 31 + (block > 1 ? 32 - __builtin_clz(block - 1) : 0);
+    const uint32_t magic = static_cast<uint32_t>(((uint64_t{1} << shift) + block - 1) / block);
+    A8Args a{q, q_stride, out, static_cast<const int*>(q_start), static_cast<const int*>(q_len), static_cast<const int*>(ctx_len), S, static_cast<const int*>(table), width, block, magic, shift, pool_rows / block,
              static_cast<const uint8_t*>(k_pool), static_cast<const uint8_t*>(v_pool), static_cast<const uint8_t*>(k_scale), static_cast<const uint8_t*>(v_scale),
              nq, nkv, d, scale * 1.4426950408889634f, window, n, few_chunk, few_chunks, static_cast<float*>(part_acc), static_cast<float*>(part_ml)};
     const long group = nq / nkv, longest = max_q_len * group;
