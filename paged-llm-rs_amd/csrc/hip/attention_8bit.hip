@@ -28,6 +28,7 @@ typedef __attribute__((address_space(3))) a8_bf16x4 a8_lds_bf16x4;
 
 #define A8_KEYS 32       // keys a wave's tile where every wave has keys of its own
 #define A8_WAVES 4
+#define A8_MOST_KEYS 2048   // of a share of few rows
 
 union a8_frag {
     a8_bf16x8 vec;
@@ -102,7 +103,8 @@ __device__ __forceinline__ void a8_split(const float (&x)[8], a8_frag (&to)[PIEC
 
 // Whether request s brings rows.  (One whose context is shorter than what it brings holds the rows of a padded step.)
 __device__ __forceinline__ bool a8_brings(const A8Args& a, int s) {
-    return a.q_len[s] > 0 && a.ctx_len[s] >= a.q_len[s] && a.q_start[s] >= 0 && a.q_start[s] <= a.n - a.q_len[s];
+    const int q = a.q_len[s], c = a.ctx_len[s], at = a.q_start[s];         // (all three at once)
+    return (q > 0) & (c >= q) & (at >= 0) & (at <= a.n - q);
 }
 
 // Rows that a request and key head bring are at most this many for the kernel of few rows (so many of its blocks of 16 as the registers hold, see A8Few), more for the kernel of many.
@@ -142,13 +144,6 @@ __device__ __forceinline__ int a8_shares(int lo, int hi, int chunk) { return hi 
 
 // Which of its request's pages a key is in: a division by the page size, as a product with ceil(2^shift / block), shift = 31 + ceil(log2(block)), exact below 2^31.
 __device__ __forceinline__ int a8_page_index(const A8Args& a, int key) { return static_cast<int>(static_cast<uint64_t>(static_cast<uint32_t>(key)) * a.magic >> a.shift); }
-// Where key `key` of request `seq` is in the pools, and its page.  (What the table says nothing sensible of is read from page 0.)
-__device__ __forceinline__ int a8_slot(const A8Args& a, int seq, int key, int& page) {
-    const int index = a8_page_index(a, key);
-    page = a.table[static_cast<size_t>(seq) * a.width + min(index, a.width - 1)];
-    page = static_cast<unsigned>(page) < static_cast<unsigned>(a.pages) ? page : 0;
-    return page * a.block + key - index * a.block;
-}
 // A page's power, a byte, as the number.
 __device__ __forceinline__ float a8_unit(uint32_t power) { return __uint_as_float(power << 23); }
 
@@ -202,12 +197,35 @@ __global__ __launch_bounds__(A8_WAVES * PL_WAVE, PIECES * RB * DQ > 6 || (PIECES
     const int k_begin = max(lo, k_base), k_end = min(hi, k_base + a.chunk);
     const int last_from = pl_first_visible(start + q_len - 1, a.window);     // (the last token's first key: no token's is later)
 
-    // Where the keys of the share are, and in what units.  (Keys that no row sees are read at the nearest one's place.)
-    for (int i = tid; i < a.chunk; i += A8_WAVES * PL_WAVE) {
-        int page;
-        slots[i] = a8_slot(a, seq, min(max(k_base + i, k_begin), k_end - 1), page);
-        const size_t at = static_cast<size_t>(page) * a.nkv + kvh;
-        units[i] = static_cast<uint16_t>(a.k_scale[at] | a.v_scale[at] << 8);
+    // Where the keys of the share are, and in what units.  (Keys that no row sees are read at the nearest one's place.)  All pages are asked for, then all powers: one behind the other they would be a
+    // wait each for every 256 keys.
+    constexpr int EACH = A8_MOST_KEYS / (A8_WAVES * PL_WAVE);
+    const int keys = min(pl_ceil_div(k_end - k_base, A8_KEYS) * A8_KEYS, a.chunk);
+    int page[EACH];
+    const int* row_table = a.table + static_cast<size_t>(seq) * a.width;
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) {
+        const int i = tid + e * A8_WAVES * PL_WAVE;
+        if (e * A8_WAVES * PL_WAVE < keys) page[e] = row_table[min(a8_page_index(a, min(max(k_base + i, k_begin), k_end - 1)), a.width - 1)];
+    }
+    uint32_t k_power[EACH], v_power[EACH];
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) {
+        if (e * A8_WAVES * PL_WAVE < keys) {
+            page[e] = static_cast<unsigned>(page[e]) < static_cast<unsigned>(a.pages) ? page[e] : 0;
+            const size_t at = static_cast<size_t>(page[e]) * a.nkv + kvh;
+            k_power[e] = a.k_scale[at];
+            v_power[e] = a.v_scale[at];
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) {
+        const int i = tid + e * A8_WAVES * PL_WAVE;
+        if (i < keys) {
+            const int key = min(max(k_base + i, k_begin), k_end - 1);
+            slots[i] = page[e] * a.block + key - a8_page_index(a, key) * a.block;
+            units[i] = static_cast<uint16_t>(k_power[e] | v_power[e] << 8);
+        }
     }
 
     // The rows: what a lane reads of a key with its j-th load are the values 64 j + 16 quarter .. + 15, two operands
@@ -241,39 +259,48 @@ __global__ __launch_bounds__(A8_WAVES * PL_WAVE, PIECES * RB * DQ > 6 || (PIECES
         for (int t = 0; t < 4 * DQ; ++t) acc[b][t] = a8_f32x4{0.f, 0.f, 0.f, 0.f};
     }
 
-    // A tile on its way: keys in two halves of 16, values 16 bytes a lane, 4 DQ lanes a key
+    // A tile on its way: keys in two halves of 16, values 16 bytes a lane, 4 DQ lanes a key.  Where they are is read from LDS a tile before their bytes are asked for, and no load stands under a condition
+    // (a lane without a piece of a head reads the last one: the queries' zeros take its products out, and nothing keeps its results), so a tile has no wait but for its bytes.
     constexpr int VP = 4 * DQ, LOADS = 2 * DQ;
     a8_u32x4 kraw[LOADS], vraw[LOADS];
-    const size_t row_bytes = static_cast<size_t>(a.nkv) * a.d;
-    const uint8_t *k_from = a.k_pool + static_cast<size_t>(kvh) * a.d, *v_from = a.v_pool + static_cast<size_t>(kvh) * a.d;
+    int k_slot[2], v_slot[LOADS];
+    uint32_t k_unit[2], v_unit[LOADS];
+    const uint32_t row_bytes = a.nkv * a.d;
+    const int last_piece = a.d / 16 - 1;
+    const uint8_t *k_from = a.k_pool + kvh * a.d, *v_from = a.v_pool + kvh * a.d;
+    auto look = [&](int base) {
+#pragma unroll
+        for (int half = 0; half < 2; ++half) k_slot[half] = slots[base + 16 * half + col];
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) v_slot[i] = slots[base + (i * PL_WAVE + lane) / VP];
+    };
     auto fetch = [&](int base) {
 #pragma unroll
-        for (int i = 0; i < LOADS; ++i) {
-            const int at = i * PL_WAVE + lane, piece = at % VP;
-            vraw[i] = a8_u32x4{0u, 0u, 0u, 0u};
-            if (16 * piece < a.d) vraw[i] = *reinterpret_cast<const a8_u32x4*>(v_from + slots[base + at / VP] * row_bytes + 16 * piece);
-        }
+        for (int i = 0; i < LOADS; ++i) vraw[i] = *reinterpret_cast<const a8_u32x4*>(v_from + static_cast<size_t>(v_slot[i]) * row_bytes + 16 * min((i * PL_WAVE + lane) % VP, last_piece));
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            const uint8_t* from = k_from + slots[base + 16 * half + col] * row_bytes;
+        for (int half = 0; half < 2; ++half)
 #pragma unroll
-            for (int j = 0; j < DQ; ++j) {
-                const int at = 64 * j + 16 * quarter;
-                kraw[half * DQ + j] = a8_u32x4{0u, 0u, 0u, 0u};
-                if (at < a.d) kraw[half * DQ + j] = *reinterpret_cast<const a8_u32x4*>(from + at);
-            }
-        }
+            for (int j = 0; j < DQ; ++j)
+                kraw[half * DQ + j] = *reinterpret_cast<const a8_u32x4*>(k_from + static_cast<size_t>(k_slot[half]) * row_bytes + 16 * min(4 * j + quarter, last_piece));
+#pragma unroll
+        for (int half = 0; half < 2; ++half) k_unit[half] = units[base + 16 * half + col];
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) v_unit[i] = units[base + (i * PL_WAVE + lane) / VP];
     };
-    // this wave's first and last tiles with keys
+    // this wave's first and last tiles with keys (past the share's last tile that one is read once more)
     const int first_tile = (k_begin - k_base) / A8_KEYS, end_tile = pl_ceil_div(k_end - k_base, A8_KEYS);
     int tile = first_tile + wave;
-    if (tile < end_tile) fetch(tile * A8_KEYS);
+    if (tile < end_tile) {
+        look(tile * A8_KEYS);
+        fetch(tile * A8_KEYS);
+        look(min(tile + A8_WAVES, end_tile - 1) * A8_KEYS);
+    }
     for (; tile < end_tile; tile += A8_WAVES) {
-        const int base = tile * A8_KEYS, k0 = k_base + base;
+        const int k0 = k_base + tile * A8_KEYS;
 #pragma unroll
         for (int i = 0; i < LOADS; ++i) {
             const int at = i * PL_WAVE + lane, key = at / VP, piece = at % VP;
-            const float unit = a8_unit(units[base + key] >> 8);
+            const float unit = a8_unit(v_unit[i] >> 8);
             a8_frag to[2];
 #pragma unroll
             for (int e = 0; e < 4; ++e) to[e / 2].half[e % 2] = a8_widen4(vraw[i][e], unit);
@@ -284,7 +311,7 @@ __global__ __launch_bounds__(A8_WAVES * PL_WAVE, PIECES * RB * DQ > 6 || (PIECES
         a8_f32x4 s[RB][2];
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-            const float unit = a8_unit(units[base + 16 * half + col] & 0xff);
+            const float unit = a8_unit(k_unit[half] & 0xff);
 #pragma unroll
             for (int b = 0; b < RB; ++b) s[b][half] = a8_f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -298,7 +325,8 @@ __global__ __launch_bounds__(A8_WAVES * PL_WAVE, PIECES * RB * DQ > 6 || (PIECES
                     for (int p = PIECES - 1; p >= 0; --p) s[b][half] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf.vec, qf[b][j][p].vec, s[b][half], 0, 0, 0);
             }
         }
-        if (tile + A8_WAVES < end_tile) fetch((tile + A8_WAVES) * A8_KEYS);
+        fetch(min(tile + A8_WAVES, end_tile - 1) * A8_KEYS);
+        look(min(tile + 2 * A8_WAVES, end_tile - 1) * A8_KEYS);
         const bool whole = k0 >= k_begin && k0 >= last_from && k0 + A8_KEYS <= k_end && k0 + A8_KEYS - 1 <= start;
         a8_frag pf[RB][PIECES];
 #pragma unroll
@@ -331,12 +359,12 @@ __global__ __launch_bounds__(A8_WAVES * PL_WAVE, PIECES * RB * DQ > 6 || (PIECES
             for (int t = 0; t < 4 * DQ; ++t) acc[b][t] *= alpha;
         }
         __builtin_amdgcn_wave_barrier();
-        const uint16_t* from = mine + (4 * quarter + col / 4) * VROW + 4 * (col % 4);
+        const uint16_t* v_at = mine + (4 * quarter + col / 4) * VROW + 4 * (col % 4);
 #pragma unroll
         for (int t = 0; t < 4 * DQ; ++t) {
             a8_frag vf;
-            vf.half[0] = a8_read_transposed(from + 16 * t);
-            vf.half[1] = a8_read_transposed(from + 16 * VROW + 16 * t);
+            vf.half[0] = a8_read_transposed(v_at + 16 * t);
+            vf.half[1] = a8_read_transposed(v_at + 16 * VROW + 16 * t);
 #pragma unroll
             for (int b = 0; b < RB; ++b)
 #pragma unroll
@@ -825,7 +853,7 @@ extern "C" int pl_paged_attention_8bit(const void* q, int q_stride, void* out, c
     PL_REQUIRE(S >= 1 && n >= 1 && max_q_len >= 1 && min_q_len <= max_q_len && width >= 1 && block >= 1 && pool_rows >= block,
                "8-bit attention: %d requests, %d rows, %d to %d of one request, tables of %d pages of %d, %d rows", S, n, min_q_len, max_q_len, width, block, pool_rows);
     PL_REQUIRE(static_cast<long>(n) * nq < (1l << 31) && static_cast<long>(S) * nkv < (1l << 31), "8-bit attention: %d rows of %d heads, %d requests are too many for a launch", n, nq, S);
-    PL_REQUIRE(few_chunk >= A8_KEYS && few_chunk % A8_KEYS == 0 && few_chunk <= 2048 && few_chunks >= 1 && few_chunks < 65536 && (few_chunks == 1 || (part_acc && part_ml)),
+    PL_REQUIRE(few_chunk >= A8_KEYS && few_chunk % A8_KEYS == 0 && few_chunk <= A8_MOST_KEYS && few_chunks >= 1 && few_chunks < 65536 && (few_chunks == 1 || (part_acc && part_ml)),
                "8-bit attention: %d shares of %d keys", few_chunks, few_chunk);
     PL_REQUIRE(many_chunk >= 64 && many_chunk % 64 == 0 && many_chunks >= 1 && many_chunks < 65536 && (many_chunks == 1 || (part_acc && part_ml)),
                "8-bit attention: %d shares of %d keys", many_chunks, many_chunk);
