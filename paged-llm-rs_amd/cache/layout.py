@@ -107,7 +107,12 @@ class CacheLayout:
         return sum((1 if g.spec.values_in_keys else 2) * len(g.layers) * g.spec.kv_heads * g.spec.head_dim * element_size
                    for g in self.groups)
 
-    def blocks_within(self, budget_bytes: int, block_size: int, element_size: int) -> int:
-        """Pages a byte budget holds, at least one (reference: batch.rs:54-57)."""
-        per_block = block_size * self.bytes_per_token(element_size)
+    @property
+    def power_bytes(self) -> int:
+        """Bytes that the powers of two of one page take over all layers, where pages are held in 8 bits."""
+        return sum(2 * len(g.layers) * g.spec.kv_heads for g in self.groups)
+
+    def blocks_within(self, budget_bytes: int, block_size: int, element_size: int, beside: int = 0) -> int:
+        """Pages a byte budget holds, at least one (reference: batch.rs:54-57).  ``beside``: bytes that a page takes besides its tokens'."""
+        per_block = block_size * self.bytes_per_token(element_size) + beside
         return max(budget_bytes // max(per_block, 1), 1)

@@ -1,6 +1,7 @@
 """The device side of the cache: for every layer that owns pages a key pool and
 a value pool, [pages * page size, kv_heads * head_dim], allocated once and never
-grown (reference: batch.rs:279-315); and for every layer with per-request state
+grown (reference: batch.rs:279-315), in the model's type or in e4m3 with a power of
+two for every page and key head beside each; and for every layer with per-request state
 a tensor [slots, ...].  Page numbers are shared by the layers of a group.
 """
 
@@ -24,11 +25,14 @@ class LayerKV:
     block_table: torch.Tensor   # [requests of the step, pages a request], -1 where there is none
     block_size: int
     group: int
+    k_scale: torch.Tensor | None = None    # pages held in 8 bits: the powers of two of their keys and values [pages, key heads]
+    v_scale: torch.Tensor | None = None
 
 
 class PagedCache:
     def __init__(self, layout: CacheLayout, block_size: int, num_blocks: int, dtype: torch.dtype,
-                 device, max_seqs: int = 64):
+                 device, max_seqs: int = 64, eight_bit: bool = False):
+        """``eight_bit``: pages of e4m3 with a power of two a page and key head, whatever the model's type (``kernels.qk_norm_rope_kv_write_8bit``)."""
         if block_size < 1:
             raise ConfigError(f"block size {block_size}, which has to be at least one")
         if num_blocks < 1:
@@ -43,10 +47,17 @@ class PagedCache:
                     for g in layout.groups]
         self.manager = CacheManager(geometry, state_slots=max_seqs if layout.states else 0)
         self._pools: dict = {}
+        self._powers: dict = {}
+        if eight_bit and any(g.spec.values_in_keys for g in layout.groups):
+            raise ConfigError("layers whose values are read out of their keys keep no pages in 8 bits")
         for g in layout.groups:
             width = g.spec.kv_heads * g.spec.head_dim
             for layer in g.layers:
-                keys = torch.zeros((num_blocks * block_size, width), dtype=dtype, device=self.device)
+                keys = torch.zeros((num_blocks * block_size, width), dtype=kernels.E4M3 if eight_bit else dtype, device=self.device)
+                if eight_bit:
+                    # (2^0 until a page is begun)
+                    self._powers[layer] = tuple(torch.full((num_blocks, g.spec.kv_heads), 127, dtype=torch.uint8, device=self.device).view(kernels.E8M0)
+                                                for _ in range(2))
                 # (a layer whose values are read out of its keys' rows has the one pool in both places)
                 values = keys if g.spec.values_in_keys else torch.zeros_like(keys)
                 self._pools[layer] = (keys, values)
@@ -58,14 +69,15 @@ class PagedCache:
 
     @property
     def bytes(self) -> int:
-        return sum(k.numel() * k.element_size() * (1 if v is k else 2) for k, v in self._pools.values())
+        return (sum(k.numel() * k.element_size() * (1 if v is k else 2) for k, v in self._pools.values())
+                + sum(p.numel() for pair in self._powers.values() for p in pair))
 
     def layer_view(self, layer: int, batch) -> LayerKV:
         if layer not in self._pools:
             raise ConfigError(f"layer {layer} owns no pages")
         group = self.layout.layer_group[layer]
         k, v = self._pools[layer]
-        return LayerKV(k, v, batch.block_tables[group], self.block_size, group)
+        return LayerKV(k, v, batch.block_tables[group], self.block_size, group, *self._powers.get(layer, (None, None)))
 
     def layer_pools(self, layer: int):
         return self._pools[layer]

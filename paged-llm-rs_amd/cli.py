@@ -28,6 +28,9 @@ def parser() -> argparse.ArgumentParser:
     p.add_argument("--max-tokens", type=int, default=512, help="token budget for a request that names none")
     p.add_argument("--block-size", type=int, default=16, help="tokens per cache block")
     p.add_argument("--cache-mib", type=int, default=3584, help="bytes the KV cache may take, in mebibytes")
+    p.add_argument("--cache-dtype", default="auto", choices=["auto", "e4m3"],
+                   help="what the KV cache holds: the model's type, or 8 bits a value with a power of two a block and head "
+                        "(twice the tokens of bf16 in the same bytes; plain attention layers only)")
     p.add_argument("--max-batch", type=int, default=16, help="rows in one decode pass")
     p.add_argument("--attention", default="kernel", choices=["tensor", "kernel"],
                    help="kernel: the matrix-core attention kernels; tensor: the plain 32-bit-arithmetic kernel "
@@ -107,7 +110,8 @@ def main(argv=None) -> int:
         kernels.set_attention(args.attention)
         engine = Engine(args.model, dtype=args.dtype, block_size=args.block_size, cache_mib=args.cache_mib,
                         max_batch=args.max_batch, chunk=chunk, prefix_cache=args.prefix_cache == "on",
-                        max_tokens=args.max_tokens, sampler=args.sampler, strips=args.strips == "on")
+                        max_tokens=args.max_tokens, sampler=args.sampler, strips=args.strips == "on",
+                        cache_dtype=args.cache_dtype)
         print(engine.describe(), file=sys.stderr, flush=True)
         if not prompts:
             return 0

@@ -71,6 +71,12 @@ class Engine:
     the budget of a request that names none).  ``num_blocks`` sets the pool
     directly instead of ``cache_mib``.
 
+    ``cache_dtype``: what the pages hold, ``auto`` (the model's type) or ``e4m3``: keys and values in 8 bits with a power of two a page and
+    key head, so the same ``cache_mib`` holds twice the tokens of bfloat16 (four times those of 32 bits) and decoding reads half
+    the bytes.  For models all of whose layers with pages are the plain attention with heads of a multiple of 16.  What is
+    read back is rounded to four bits of a value, and again when a page's largest value outgrows what it held, so the logits are not those of a
+    cache in the model's type, and their last bits depend on how a prompt was cut into portions.
+
     ``strips``: the weights are kept a second time in the order the products of a decoding step read them
     fastest (``kernels.weights_in_strips``), which costs their memory again.
 
@@ -84,7 +90,7 @@ class Engine:
     def __init__(self, model, dtype: str = "auto", block_size: int = 16, cache_mib: int = 3584,
                  num_blocks: Optional[int] = None, max_batch: int = 16, chunk=128, prefix_cache: bool = True,
                  max_tokens: int = 512, device="cuda:0", sampler: str = "device", graphs: bool = True,
-                 ahead: bool = True, strips: bool = True):
+                 ahead: bool = True, strips: bool = True, cache_dtype: str = "auto"):
         self.device = require_gpu(device)
         dtype = {"auto": None, "f32": "float32", "bf16": "bfloat16"}.get(dtype, dtype)
         if dtype is None:
@@ -97,20 +103,29 @@ class Engine:
             raise ConfigError("--chunk 0 would carry nothing")
         if sampler not in ("device", "host"):
             raise ConfigError(f"sampler {sampler!r}, which is neither device nor host")
+        if cache_dtype not in ("auto", "e4m3"):
+            raise ConfigError(f"cache dtype {cache_dtype!r}, which is neither auto nor e4m3")
         self.dtype = dtype
+        self.cache_dtype = dtype if cache_dtype == "auto" else cache_dtype
         self.model_dir = Path(model)
         self.config, self.model = load_model(model, dtype, self.device, strips=strips)
         self.generation = GenerationConfig.from_dir(model)
         element = 4 if dtype == "float32" else 2
         layout = self.model.cache_layout
+        eight_bit = cache_dtype == "e4m3"
+        if eight_bit:
+            mixers = [m for m in (getattr(b, "mixer", None) for b in self.model.blocks) if m is not None and m.cache_spec() is not None]
+            if not mixers or not all(getattr(m, "takes_8bit_pages", False) for m in mixers):
+                raise ConfigError("cache dtype e4m3: not every layer with pages is plain attention with heads of a multiple of 16")
+            element = 1
         if num_blocks is None:
             # The page count follows from the byte budget, so changing the page
             # size compares two layouts at the same memory (reference: main.rs:89-120).
-            num_blocks = layout.blocks_within(int(cache_mib) << 20, block_size, element)
+            num_blocks = layout.blocks_within(int(cache_mib) << 20, block_size, element, layout.power_bytes if eight_bit else 0)
         self.block_size, self.num_blocks = block_size, num_blocks
         self.bytes_per_token = layout.bytes_per_token(element)
         self.cache = PagedCache(layout, block_size, num_blocks, DTYPES[dtype], self.device,
-                                max_seqs=max(max_batch * 2, 8))
+                                max_seqs=max(max_batch * 2, 8), eight_bit=eight_bit)
         self.scheduler = sched.Scheduler(self.cache.manager, max_batch=max_batch,
                                          chunk=None if chunk is None else int(chunk),
                                          max_positions=self.model.spec.max_positions, prefix_cache=prefix_cache)
@@ -324,7 +339,7 @@ class Engine:
             f"  sampling temperature {self.generation.temperature}, top_p {self.generation.top_p}, "
             f"top_k {self.generation.top_k}, from the model's generation config\n"
             f"  stop     {self.generation.eos_token_ids}\n"
-            f"  cache    {self.num_blocks} blocks of {self.block_size} tokens, "
+            f"  cache    {self.num_blocks} blocks of {self.block_size} tokens in {self.cache_dtype}, "
             f"{self.cache.bytes / 2 ** 30:.2f} GiB, {self.bytes_per_token} bytes a token, "
             f"{self.num_blocks * self.block_size} tokens held at once, prefix cache {self.prefix_cache}")
 

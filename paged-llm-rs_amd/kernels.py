@@ -2940,12 +2940,17 @@ class StepTables(NamedTuple):
 def _fits(t: torch.Tensor, what: str, dtype: torch.dtype, count: int, device: int, shape=None) -> int:
     """The address of a tensor of ``count`` values that the launch can take: of this type, contiguous, on the current device (launches go to its stream, and a tensor of
     another device would be read from there).  Asked for in few words, since a step of single tokens is as long as its launches take the host."""
-    if t.dtype is not dtype or t.get_device() != device or t.numel() != count or not t.is_contiguous() or (shape is not None and tuple(t.shape) != shape):
+    if t.dtype is not dtype or t.get_device() != device or t.numel() != count or not t.is_contiguous() or (shape is not None and t.shape != shape):
         _need(t, what, shape, dtype)
         if t.get_device() != device:
             raise TensorError(f"{what} is on {t.device}, the current device is cuda:{device}")
         raise TensorError(f"{what} has shape {tuple(t.shape)}, expected {count} values")
     return t.data_ptr()
+
+
+def _stream_of(device: int) -> int:
+    """The handle of torch's current stream on ``device``, the current one."""
+    return _raw_stream(device) if _raw_stream is not None else _stream()
 
 
 def step_tables(q_len: torch.Tensor, ctx_len: torch.Tensor, block_table: torch.Tensor, block_size: int, free_pages: torch.Tensor | None, rows: int) -> StepTables:
@@ -2979,7 +2984,7 @@ def step_tables(q_len: torch.Tensor, ctx_len: torch.Tensor, block_table: torch.T
     made = StepTables(*room.split_with_sizes([rows, rows, rows, S, 1]))
     at = room.data_ptr()
     _check(library().pl_step_tables(brings, context, S, table, width, block_size, free, count, rows, at + 12 * rows, at, at + 4 * rows, at + 8 * rows, at + 12 * rows + 4 * S,
-                                    _stream()))
+                                    _stream_of(device)))
     return made
 
 
@@ -3036,9 +3041,10 @@ def qk_norm_rope_kv_write_8bit(qkv: torch.Tensor, q: torch.Tensor | None, q_gain
     places = _fits(slots, "slots", torch.int32, n, device) if write_kv else 0
     _check(library().pl_qk_norm_rope_kv_write_8bit(
         source, queries, stride, q_gains, k_gains, gain_code, eps, cosines, sines, rot, angles, 1 if neighbours else 0, _fits(positions, "positions", torch.int32, n, device), places,
-        block_size, rows, keys, values, key_powers, value_powers, n, nq, nkv, d, code, _stream()))
+        block_size, rows, keys, values, key_powers, value_powers, n, nq, nkv, d, code, _stream_of(device)))
 
 
+@functools.lru_cache(maxsize=4096)
 def shares_8bit(n: int, requests: int, max_ctx: int, nq: int, nkv: int, window: int = 0) -> tuple:
     """(keys a share, shares) of the 8-bit attention's kernel of few rows, and the same of its kernel of many.
 
@@ -3098,5 +3104,24 @@ def paged_attention_8bit(q: torch.Tensor, q_row_stride: int, out: torch.Tensor, 
     _check(library().pl_paged_attention_8bit(
         queries, q_row_stride, results, _fits(q_start, "first row of each request", torch.int32, S, device), _fits(q_len, "tokens of each request", torch.int32, S, device),
         _fits(ctx_len, "context length of each request", torch.int32, S, device), S, n, max_q_len, min_q_len, _fits(block_table, "block table", torch.int32, S * width, device), width,
-        block_size, rows, keys, values, key_powers, value_powers, nq, nkv, d, scale, window, few, few_shares, many, many_shares, acc, ml, code, _stream()))
+        block_size, rows, keys, values, key_powers, value_powers, nq, nkv, d, scale, window, few, few_shares, many, many_shares, acc, ml, code, _stream_of(device)))
     return out
+
+
+def step_slots(batch, kv) -> torch.Tensor:
+    """The slot of every row of a step in one group of pages (-1: a row of padding), from the lengths and the table that the step carries."""
+    return step_tables(batch.q_len, batch.ctx_len, kv.block_table, kv.block_size, None, batch.num_tokens).slots
+
+
+def attention_step_8bit(qkv: torch.Tensor, out: torch.Tensor, batch, kv, slots: torch.Tensor, nq: int, nkv: int, d: int, scale: float, window: int,
+                        prepare: QkFusion) -> torch.Tensor:
+    """What ``attention_step`` does, over pages held in 8 bits: ``slots`` from ``step_slots``."""
+    if _attention_mode != "kernel":
+        raise TensorError("the plain attention kernel reads no pages held in 8 bits")
+    qk_norm_rope_kv_write_8bit(qkv, None, prepare.q_gain, prepare.k_gain, prepare.eps, prepare.cos, prepare.sin, prepare.rot, batch.positions, slots, kv.block_size, kv.k_pool,
+                               kv.v_pool, kv.k_scale, kv.v_scale, nq, nkv, d, neighbours=prepare.neighbours, write_kv=prepare.write_kv)
+    # (A padded step reports bounds that hold for every step of its shape.  Whether there are short requests is part of a shape; how near the contexts are is one of bfloat16's.)
+    shortest = int(batch.tokens_each.min()) if not batch.padded else SHORT_PORTION if batch.tokens_of_short_requests(SHORT_PORTION) == 0 else 1
+    return paged_attention_8bit(qkv, qkv.shape[1], out, batch.q_start, batch.q_len, batch.ctx_len, batch.max_q_len,
+                                batch.near_ctx_len if qkv.dtype == torch.bfloat16 else batch.max_ctx_len, kv.block_table, kv.block_size, kv.k_pool, kv.v_pool, kv.k_scale,
+                                kv.v_scale, nq, nkv, d, scale, window, min_q_len=min(shortest, batch.max_q_len))

@@ -94,10 +94,29 @@ class PagedAttention:
         return self.o_proj.forward(out, add_into=ctx.residual,
                                    hand=getattr(ctx, "hand", None) if ctx.residual is not None else None)
 
+    @property
+    def takes_8bit_pages(self) -> bool:
+        """Whether this mixer's pages may be held in 8 bits (``cache_dtype``)."""
+        return type(self).attend is PagedAttention.attend and self.d % 16 == 0
+
+    def _attend_8bit(self, x, ctx, kv, projected):
+        """The same over pages held in 8 bits: one kernel more in front of the attention, and one a step that works out where the tokens go."""
+        batch = ctx.batch
+        qkv = projected if projected is not None else self.qkv_proj.forward(x)
+        where = ("slots of the pages", kv.group)
+        if where not in ctx.carried:
+            ctx.carried[where] = kernels.step_slots(batch, kv)
+        out = torch.empty((qkv.shape[0], self.nq * self.d), dtype=qkv.dtype, device=qkv.device)
+        if ctx.trace is not None:
+            self._record_projections(qkv, batch, kv, ctx.trace)
+        return kernels.attention_step_8bit(qkv, out, batch, kv, ctx.carried[where], self.nq, self.nkv, self.d, self.scale, self.window, self._prepare(ctx.writes_cache))
+
     def attend(self, x, ctx, projected=None):
         """Everything before the output projection.  ``projected``: the rows of q, k and v, where the layer before has worked them out."""
         batch = ctx.batch
         kv = ctx.kv()
+        if getattr(kv, "k_scale", None) is not None:
+            return self._attend_8bit(x, ctx, kv, projected)
         prepare = self._prepare(ctx.writes_cache)
         # (many rows: the projection may do what stands between it and attention, unless one kernel does that and the attention)
         qkv = None
@@ -121,7 +140,7 @@ class PagedAttention:
 
     def chain_attention(self, batch, kv, writes_cache: bool):
         """This layer's attention as the last stage of the launch before it (``kernels.ChainAttention``), where it may be that."""
-        if type(self).attend is not PagedAttention.attend:
+        if type(self).attend is not PagedAttention.attend or getattr(kv, "k_scale", None) is not None:
             return None
         return kernels.ChainAttention.of(batch, kv, self.nq, self.nkv, self.d, self.scale, self.window, self._prepare(writes_cache))
 
@@ -152,6 +171,11 @@ class PagedAttention:
             return
         for name, heads, count, gain in (("q_norm.out", q, self.nq, self.q_gain), ("k_norm.out", k, self.nkv, self.k_gain)):
             copy = torch.cat([heads, k, v], dim=1).contiguous()
+            if getattr(kv, "k_scale", None) is not None:
+                kernels.qk_norm_rope_kv_write_8bit(copy, None, gain, gain, self.eps, None, None, 0, batch.positions, None, kv.block_size, kv.k_pool, kv.v_pool, kv.k_scale, kv.v_scale,
+                                                   count, self.nkv, self.d, write_kv=False)
+                trace.record(name, copy[:, :count * self.d])
+                continue
             kernels.qk_norm_rope_kv_write(copy, gain, gain, self.eps, None, None, 0, batch.positions, batch.seq_of,
                                           kv.block_table, kv.block_size, kv.k_pool, kv.v_pool, count, self.nkv, self.d,
                                           write_kv=False)
