@@ -624,23 +624,24 @@ __global__ __launch_bounds__(NW * PL_WAVE) __attribute__((amdgpu_waves_per_eu(NW
             if (!whole(k0 + TILE)) mask(next, k0 + TILE);
             top = largest(next);
             const uint16_t* v_from = values + (v_now * TILE + 4 * half + lane % 16 / 4) * VROW + 16 * (lane / 16 % 2) + 4 * (lane % 4);
+            // (In this order, AHEAD reads before the product that needs the first: left to itself the compiler waits for every pair of them.  Other instructions may move across.)
+            constexpr int PRODUCTS = 2 * KB * DT, AHEAD = PRODUCTS < 6 ? PRODUCTS : 6;
+            a8_frag vf[AHEAD];
+            auto read_values = [&](int i) {
+                const uint16_t* at = v_from + 16 * (i / DT) * VROW + 32 * (i % DT);
+                vf[i % AHEAD].half[0] = a8_read_transposed(at);
+                vf[i % AHEAD].half[1] = a8_read_transposed(at + 8 * VROW);
+            };
 #pragma unroll
-            for (int g = 0; g < 2 * KB; ++g)
+            for (int i = 0; i < AHEAD; ++i) read_values(i);
 #pragma unroll
-                for (int t = 0; t < DT; ++t) {
-                    a8_frag vf;
-                    vf.half[0] = a8_read_transposed(v_from + 16 * g * VROW + 32 * t);
-                    vf.half[1] = a8_read_transposed(v_from + (16 * g + 8) * VROW + 32 * t);
+            for (int i = 0; i < PRODUCTS; ++i) {
+                __builtin_amdgcn_sched_barrier(0x6);
 #pragma unroll
-                    for (int p = PIECES - 1; p >= 0; --p) acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf.vec, pf[g][p].vec, acc[t], 0, 0, 0);
-                }
-            __builtin_amdgcn_sched_group_barrier(0x100, 6, 0);
-#pragma unroll
-            for (int i = 0; i < 2 * DT * KB; ++i) {
-                __builtin_amdgcn_sched_group_barrier(0x8, PIECES, 0);
-                __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
-                __builtin_amdgcn_sched_group_barrier(0x2, 3, 0);
+                for (int p = PIECES - 1; p >= 0; --p) acc[i % DT] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[i % AHEAD].vec, pf[i / DT][p].vec, acc[i % DT], 0, 0, 0);
+                if (i + AHEAD < PRODUCTS) read_values(i + AHEAD);
             }
+            __builtin_amdgcn_sched_barrier(0x6);
         } else if (sees(k0 + TILE)) {
             scores(next, (t + 1) % 2);
             mask(next, k0 + TILE);
