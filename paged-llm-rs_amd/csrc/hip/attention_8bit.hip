@@ -438,9 +438,10 @@ __global__ __launch_bounds__(A8_WAVES * PL_WAVE, PIECES * RB * DQ > 6 || (PIECES
 // What bounds it is the weights: an exponential takes a wave four times as long as another vector instruction, and together they take as long as the products.  So the scores of the next tile are multiplied while
 // the weights of this one are made, and the next maximum is found while this tile's weights meet its values: both pipes work in one wave, whatever the other waves of the unit do.
 // For that the keys in LDS are a tile ahead of the values (two lengths of keys, three of values), their bytes another tile ahead in registers, and their pages one more.  A round has one barrier.
-template <int DT>
+template <int PIECES, int DT>
 struct A8Many {
-    static constexpr int KB = DT == 8 ? 1 : 2;          // (what 160 KB of LDS hold)
+    static constexpr int KB = DT == 8 || (PIECES == 3 && DT != 4) ? 1 : 2;     // (what 160 KB of LDS hold; in 32 bits what leaves two waves a SIMD their registers, where that can be)
+    static constexpr int WAVES = PIECES == 1 ? (DT <= 4 ? 2 : 1) : (DT <= 3 ? 2 : 1);   // a SIMD
     static constexpr int KROW = 32 * DT + 8, VROW = 32 * DT + (DT % 2 == 0 ? 32 : 0);
     static constexpr size_t LDS = static_cast<size_t>(32 * KB) * (2 * KROW + 3 * VROW) * 2;
 };
@@ -452,8 +453,8 @@ __device__ __forceinline__ float a8_max_half(float v) {
 }
 
 template <int PIECES, int DT, int NW>
-__global__ __launch_bounds__(NW * PL_WAVE) __attribute__((amdgpu_waves_per_eu(NW == 8 ? 2 : 1, NW == 8 ? 2 : 1))) void attention_8bit_many_kernel(A8Args a, int few) {
-    constexpr int KB = A8Many<DT>::KB, TILE = 32 * KB, KROW = A8Many<DT>::KROW, VROW = A8Many<DT>::VROW, THREADS = NW * PL_WAVE;
+__global__ __launch_bounds__(NW * PL_WAVE) __attribute__((amdgpu_waves_per_eu(A8Many<PIECES, DT>::WAVES, A8Many<PIECES, DT>::WAVES))) void attention_8bit_many_kernel(A8Args a, int few) {
+    constexpr int KB = A8Many<PIECES, DT>::KB, TILE = 32 * KB, KROW = A8Many<PIECES, DT>::KROW, VROW = A8Many<PIECES, DT>::VROW, THREADS = NW * PL_WAVE;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     uint16_t* keys = reinterpret_cast<uint16_t*>(lds);                 // [2][TILE][KROW]
     uint16_t* values = keys + 2 * TILE * KROW;                         // [3][TILE][VROW]
@@ -489,52 +490,58 @@ __global__ __launch_bounds__(NW * PL_WAVE) __attribute__((amdgpu_waves_per_eu(NW
 
     // Tiles on their way: 16 bytes a lane and load, 2 DT lanes a key.  The pages of a tile are asked for a round before its bytes, so that no round waits for one read behind another.
     constexpr int VP = 2 * DT, LOADS = (TILE * VP + THREADS - 1) / THREADS;
-    a8_u32x4 kraw[LOADS], vraw[LOADS];
-    uint32_t kpow[LOADS], vpow[LOADS];      // (bytes as they come: made into a unit here they would be waited for here)
-    int pages[LOADS], offs[LOADS];
+    struct Bytes {
+        a8_u32x4 k[LOADS], v[LOADS];
+        uint32_t k_power[LOADS], v_power[LOADS];      // (as they come: made into a unit where they are read they would be waited for there)
+    };
+    struct Places {
+        int page[LOADS], off[LOADS];
+    };
     // (No load stands under a condition: what comes behind one is waited for where the paths meet.  A lane without a piece of a head reads the last one, whose products the queries' zeros take out.)
     const int last_piece = a.d / 16 - 1;
-    auto look = [&](int k0) {
+    auto look = [&](int k0, Places& to) {
 #pragma unroll
         for (int i = 0; i < LOADS; ++i) {
             const int at = i * THREADS + tid;
             const int key = min(max(k0 + at / VP, k_begin), k_end - 1);      // (keys that no row sees are read at the nearest one's place)
             const int index = a8_page_index(a, key);
-            offs[i] = key - index * a.block;
-            pages[i] = a.table[static_cast<size_t>(seq) * a.width + min(index, a.width - 1)];
+            to.off[i] = key - index * a.block;
+            to.page[i] = a.table[static_cast<size_t>(seq) * a.width + min(index, a.width - 1)];
         }
     };
-    auto fetch = [&]() {
+    auto fetch = [&](const Places& at, Bytes& to) {
 #pragma unroll
         for (int i = 0; i < LOADS; ++i) {
             const int piece = min((i * THREADS + tid) % VP, last_piece);
-            const int page = static_cast<unsigned>(pages[i]) < static_cast<unsigned>(a.pages) ? pages[i] : 0;
-            const size_t from = (static_cast<size_t>(page * a.block + offs[i]) * a.nkv + kvh) * a.d + 16 * piece;
-            kraw[i] = *reinterpret_cast<const a8_u32x4*>(a.k_pool + from);
-            vraw[i] = *reinterpret_cast<const a8_u32x4*>(a.v_pool + from);
-            kpow[i] = a.k_scale[static_cast<size_t>(page) * a.nkv + kvh];
-            vpow[i] = a.v_scale[static_cast<size_t>(page) * a.nkv + kvh];
+            const int page = static_cast<unsigned>(at.page[i]) < static_cast<unsigned>(a.pages) ? at.page[i] : 0;
+            const size_t from = (static_cast<size_t>(page * a.block + at.off[i]) * a.nkv + kvh) * a.d + 16 * piece;
+            to.k[i] = *reinterpret_cast<const a8_u32x4*>(a.k_pool + from);
+            to.v[i] = *reinterpret_cast<const a8_u32x4*>(a.v_pool + from);
+            to.k_power[i] = a.k_scale[static_cast<size_t>(page) * a.nkv + kvh];
+            to.v_power[i] = a.v_scale[static_cast<size_t>(page) * a.nkv + kvh];
         }
     };
-    auto put = [&](int k_buffer, int v_buffer) {
+    auto put = [&](const Bytes& from, int k_buffer, int v_buffer) {
 #pragma unroll
         for (int i = 0; i < LOADS; ++i) {
             const int at = i * THREADS + tid, key = at / VP, piece = at % VP;
             if (TILE * VP % THREADS != 0 && at >= TILE * VP) continue;
             a8_frag to[2];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) to[e / 2].half[e % 2] = a8_widen4(kraw[i][e], a8_unit(kpow[i]));
+            for (int e = 0; e < 4; ++e) to[e / 2].half[e % 2] = a8_widen4(from.k[i][e], a8_unit(from.k_power[i]));
             uint16_t* k_to = keys + (k_buffer * TILE + key) * KROW + 16 * piece;
             *reinterpret_cast<a8_u32x4*>(k_to) = to[0].raw;
             *reinterpret_cast<a8_u32x4*>(k_to + 8) = to[1].raw;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) to[e / 2].half[e % 2] = a8_widen4(vraw[i][e], a8_unit(vpow[i]));
+            for (int e = 0; e < 4; ++e) to[e / 2].half[e % 2] = a8_widen4(from.v[i][e], a8_unit(from.v_power[i]));
             uint16_t* v_to = values + (v_buffer * TILE + key) * VROW + 16 * piece;
             *reinterpret_cast<a8_u32x4*>(v_to) = to[0].raw;
             *reinterpret_cast<a8_u32x4*>(v_to + 8) = to[1].raw;
         }
     };
 
+    Bytes bytes;
+    Places places;
     a8_f32x16 acc[DT];
 #pragma unroll
     for (int t = 0; t < DT; ++t)
@@ -647,23 +654,27 @@ __global__ __launch_bounds__(NW * PL_WAVE) __attribute__((amdgpu_waves_per_eu(NW
             mask(next, k0 + TILE);
             top = largest(next);
         }
-        put(t % 2, v_put);
-        fetch();
-        look(k0 + 4 * TILE);
+        put(bytes, t % 2, v_put);
+        fetch(places, bytes);
+        look(k0 + 4 * TILE, places);
         v_now = v_now == 2 ? 0 : v_now + 1;
         __syncthreads();
     };
 
     // (beyond the last tile the nearest key is read once more: no round goes by whether there is a next one)
-    look(k_first);
-    fetch();
-    look(k_first + TILE);
-    put(0, 0);
-    fetch();
-    look(k_first + 2 * TILE);
-    put(1, 1);
-    fetch();
-    look(k_first + 3 * TILE);
+    {
+        Places second;
+        Bytes first;
+        look(k_first, places);
+        look(k_first + TILE, second);
+        fetch(places, first);
+        look(k_first + 2 * TILE, places);
+        fetch(second, bytes);
+        put(first, 0, 0);
+        put(bytes, 1, 1);
+        fetch(places, bytes);
+        look(k_first + 3 * TILE, places);
+    }
     __syncthreads();
     a8_f32x16 s[2][KB];
     if (sees(k_first)) {
@@ -803,7 +814,7 @@ static int launch_few(const A8Args& a, int rows, hipStream_t stream) {
 
 template <int PIECES, int DT, int NW>
 static int launch_many(const A8Args& a, int few, long blocks, hipStream_t stream) {
-    const size_t lds = A8Many<DT>::LDS;
+    const size_t lds = A8Many<PIECES, DT>::LDS;
     if (int e = a8_lds(reinterpret_cast<const void*>(&attention_8bit_many_kernel<PIECES, DT, NW>), lds)) return e;
     PL_REQUIRE(blocks * a.nkv < (1l << 31), "8-bit attention: %ld blocks of rows are too many for a launch", blocks);
     attention_8bit_many_kernel<PIECES, DT, NW><<<dim3(static_cast<unsigned>(blocks * a.nkv), a.chunks), NW * PL_WAVE, lds, stream>>>(a, few);
