@@ -6,6 +6,7 @@
 // step of the last unit plus half a step of every finer one before, less than a whole step).  It never shrinks before the page is begun anew.
 // A power of two and not any scale: e4m3 times a power of two is exact in bfloat16 and in 32 bits, so reading rounds nothing.
 #include "common.hpp"
+#include "head_rows.hpp"
 
 #define P8_LARGEST_SEQS 8192      // two words of LDS a request: 64 KB
 #define P8_TABLE_THREADS 256
@@ -204,8 +205,12 @@ struct P8Turn {
             float ss = 0.f;
 #pragma unroll
             for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], ss);
+            if constexpr (LPR == 16) {
+                ss = hr_sum16(ss);
+            } else {
 #pragma unroll
-            for (int off = LPR / 2; off > 0; off >>= 1) ss += __shfl_xor(ss, off, PL_WAVE);
+                for (int off = LPR / 2; off > 0; off >>= 1) ss += __shfl_xor(ss, off, PL_WAVE);
+            }
             rinv = 1.f / sqrtf(ss / static_cast<float>(a.d) + a.eps);
             if (here)
 #pragma unroll
@@ -213,6 +218,16 @@ struct P8Turn {
         }
         if (a.rot == 0) return;
         if constexpr (PIECES) {
+            // (A head of 128 turned whole, the usual one: the partner is eight lanes on in the row of 16, which moves through the vector pipe and not through LDS.)
+            if (LPR == 16 && half == 64) {
+                if (!plain)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const float p = hr_dpp<0x128>(x[e]);
+                        x[e] = low ? x[e] * c[e] - p * s[e] : x[e] * c[e] + p * s[e];
+                    }
+                return;
+            }
             const int lane = threadIdx.x % PL_WAVE, other = low ? lane + half / 8 : lane - half / 8;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {

@@ -501,6 +501,79 @@ def test_requests_from_their_first_token_on(dtype):
         scene.check(out)
 
 
+def test_a_captured_step_of_all_three():
+    """Slots, write and attention of a decoding step in one graph, replayed while the contexts grow, with eager work between: the bits of the eager calls on pages of their own."""
+    from paged_llm_rs_amd import kernels
+
+    nq, nkv, d, block, S, width = 16, 8, 128, 16, 5, 40
+    ctx = i32([600, 17, 16, 1, 333])
+    brings = i32([1] * S)
+    table = i32(torch.randperm(S * width).tolist()).view(S, width)
+    pages = Pages(S * width, block, nkv, d, fill=0x30, power=121)
+    qkv = torch.randn(S, (nq + 2 * nkv) * d, device=DEV).to(torch.bfloat16)
+    gain = torch.ones(d, dtype=torch.bfloat16, device=DEV)
+    angle = torch.rand(block * width, d // 2, device=DEV) * 6
+    cos, sin = angle.cos(), angle.sin()
+
+    def step(pages, ctx, qkv, q, out):
+        made = kernels.step_tables(brings, ctx, table, block, None, S)
+        write(pages, qkv, made.slots, made.positions, nq, q=q, gains=(gain, gain), cos=cos, sin=sin, rot=d)
+        kernels.paged_attention_8bit(q, nq * d, out, made.q_start, brings, ctx, 1, block * width, table, block, *pages, nq, nkv, d, d ** -0.5)
+
+    twin = pages.clone()
+    q, out = (torch.empty(S, nq * d, dtype=torch.bfloat16, device=DEV) for _ in range(2))
+    idle = torch.zeros_like(ctx)
+    step(pages, idle, qkv, q, out)                        # (a step of padding: nothing is written)
+    assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(pages, twin))
+    static = ctx.clone()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step(pages, static, qkv, q, out)
+    for i in range(20):
+        qkv.copy_((torch.randn(S, (nq + 2 * nkv) * d, device=DEV) * 2 ** (i / 4)).to(torch.bfloat16))
+        static.copy_(ctx + i)
+        graph.replay()
+        q2, out2 = torch.empty_like(q), torch.empty_like(out)
+        step(twin, ctx + i, qkv, q2, out2)
+        if i % 3 == 0:
+            torch.cuda.synchronize()
+        assert torch.equal(q, q2) and torch.equal(out, out2), i
+        assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(pages, twin)), i
+
+
+def test_pages_behind_four_gigabytes():
+    """The same requests over the last pages of pools of 4.9 GB: the bits of a small pool."""
+    from paged_llm_rs_amd import kernels
+
+    scene = Scene(MIXES["portions"], 16, 8, 128, 16, torch.bfloat16)
+    want = scene.run()
+    total, few = 300000, scene.pages.powers[0].shape[0]
+    far = Pages(total, 16, 8, 128)
+    for big, small in zip(far, scene.pages):
+        big.view(torch.uint8)[-small.shape[0]:] = small.view(torch.uint8)
+    table = torch.where(scene.table >= 0, scene.table + (total - few), scene.table)
+    near = scene.pages
+    scene.pages, scene.table = far, table
+    assert torch.equal(scene.run(), want)
+    qkv = torch.randn(40, 3 * 8 * 128, device=DEV).to(torch.bfloat16)
+    slots = i32([3 * 16 + 5 + i for i in range(40)])
+    write(near, qkv, slots, i32(list(range(40))), 8)
+    write(far, qkv, slots + (total - few) * 16, i32(list(range(40))), 8)
+    for big, small in zip(far, near):
+        assert torch.equal(big.view(torch.uint8)[-small.shape[0]:], small.view(torch.uint8))
+    made = kernels.step_tables(scene.q_len, scene.ctx_len, table, 16, None, scene.n)
+    assert int(made.slots.max()) >= (total - few) * 16
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_attention_of_many_heads_a_key_head_and_of_a_long_context(dtype):
+    scene = Scene([(1, 300), (2, 70), (1, 1)], 300, 1, 16, 16, dtype)
+    scene.check(scene.run())
+    scene = Scene([(1, 33000), (3, 20000), (1, 12)], 8, 1, 64, 64, dtype)
+    scene.check(scene.run())
+
+
 # ---- refusals --------------------------------------------------------------------------------------------------------------------
 
 def test_refusals():
