@@ -11,6 +11,8 @@
 #define P8_LARGEST_SEQS 8192      // two words of LDS a request: 64 KB
 #define P8_TABLE_THREADS 256
 #define P8_HEADS 4                // query heads a group of lanes
+#define P8_WAVES 4
+#define P8_SINGLE_UNITS 16384     // up to so many rows times heads of keys and values every row is looked at by a wave of its own
 
 // ---- block tables and slots ---------------------------------------------------------------------------------------------
 // Request s brings q_len[s] tokens, its context behind the step is ctx_len[s]; it holds ceil((ctx - q) / block) pages and needs ceil(ctx / block).  Where new pages
@@ -135,9 +137,9 @@ extern "C" int pl_step_tables(const void* q_len, const void* ctx_len, int S, voi
 
 // ---- the write ------------------------------------------------------------------------------------------------------------
 // Rows of heads are taken eight values a lane, d / 8 lanes a row.  A run is what the step brings to one page: rows that follow each other with slots that follow
-// each other.  One workgroup takes a run of one key head, keys or values: the largest of its rows gives the page's new power, then the rows are
-// rounded into the page.  It is the workgroup of the run's first row; those of the other rows find that out from two slots and end.  Runs of more rows than the workgroup holds are read (and
-// normed, turned) twice, the second time from L2.  Queries are normed and turned by workgroups of their own in the same launch.
+// each other.  One wave or workgroup takes a run of one key head, keys or values: the largest of its rows gives the page's new power, then the rows are
+// rounded into the page.  Runs of more rows than it takes at a time are read (and normed, turned) twice, the second time from L2.  Queries are normed and turned by workgroups of their own in the
+// same launch.  Prompts are bound by what they read and write (10,503 rows of 32 + 8 heads of 128: 237 MB in 77 us, 3.1 TB/s), single tokens by the waits for slots, rows and powers one behind the other (64 of 16 + 8 heads: 5.4 us).
 struct P8Write {
     const void* qkv;
     void* q;
@@ -311,7 +313,8 @@ __device__ __forceinline__ void p8_values8(uint2 bytes, float (&x)[8]) {
 template <typename T, int LPR, int WAVES, bool PIECES>
 __device__ __forceinline__ void p8_run(const P8Write& a, int first, int slot, int head, bool keys, float* scratch) {
     constexpr int ROWS = WAVES * PL_WAVE / LPR;         // rows at a time
-    const int lane_row = threadIdx.x / LPR, chunk = threadIdx.x % LPR;
+    const int tid = WAVES == 1 ? threadIdx.x % PL_WAVE : threadIdx.x;
+    const int lane_row = tid / LPR, chunk = tid % LPR;
     const int page = slot / a.block, off = slot % a.block;
     const int source = keys ? a.nq + head : a.nq + a.nkv + head;
     uint8_t* pool = keys ? a.k_pool : a.v_pool;
@@ -360,18 +363,20 @@ __device__ __forceinline__ void p8_run(const P8Write& a, int first, int slot, in
         if (count > ROWS) p8_prepare<T, LPR, PIECES>(a, first + min(r + lane_row, count - 1), source, chunk, x);
         if (r + lane_row < count && chunk * 8 < a.d) *reinterpret_cast<uint2*>(rows + (off + r + lane_row) * row_bytes + chunk * 8) = p8_round8(x, power);
     }
-    if (threadIdx.x == 0) *scale = static_cast<uint8_t>(power);
+    if (tid == 0) *scale = static_cast<uint8_t>(power);
 }
 
-// Workgroups: first nkv * 2 a tile of `tile` rows for keys and values, then those of the queries.
+// Workgroups of four waves: first nkv * 2 units of WAVES waves a tile of `tile` rows for keys and values, then those of the queries.
 template <typename T, int LPR, int WAVES, bool PIECES>
-__global__ __launch_bounds__(WAVES * PL_WAVE) void write_8bit_kernel(P8Write a, int tile) {
-    __shared__ float scratch[WAVES];
-    constexpr int ROWS = WAVES * PL_WAVE / LPR;
+__global__ __launch_bounds__(P8_WAVES * PL_WAVE) void write_8bit_kernel(P8Write a, int tile) {
+    __shared__ float scratch[P8_WAVES];
+    constexpr int ROWS = P8_WAVES * PL_WAVE / LPR, UNITS = P8_WAVES / WAVES;
     const int tiles = a.slots != nullptr ? pl_ceil_div(a.n, tile) : 0, pairs = 2 * a.nkv;
-    const long of_pages = static_cast<long>(tiles) * pairs;
+    const long units = static_cast<long>(tiles) * pairs, of_pages = (units + UNITS - 1) / UNITS;
     if (blockIdx.x < of_pages) {
-        const int t = blockIdx.x / pairs, pair = blockIdx.x % pairs;
+        const long unit = static_cast<long>(blockIdx.x) * UNITS + (WAVES == 1 ? threadIdx.x / PL_WAVE : 0);
+        if (unit >= units) return;
+        const int t = __builtin_amdgcn_readfirstlane(static_cast<int>(unit / pairs)), pair = __builtin_amdgcn_readfirstlane(static_cast<int>(unit % pairs));
         // the first rows of runs, found by every wave for itself
         const int r = t * tile + static_cast<int>(threadIdx.x % PL_WAVE);
         const bool mine = r < min((t + 1) * tile, a.n);
@@ -412,15 +417,20 @@ __global__ __launch_bounds__(WAVES * PL_WAVE) void write_8bit_kernel(P8Write a, 
 
 template <typename T, int LPR>
 static int launch_write(const P8Write& a, hipStream_t stream) {
-    constexpr int WAVES = 4, ROWS = WAVES * PL_WAVE / LPR;
-    // A workgroup looks through `tile` rows for the first ones of runs.  One each while all of a step's may be first (decoding); with so many rows that most of them are inside a page 16, since
-    // a workgroup that finds nothing still costs its start (8,100 rows of prompts into 8 heads: TILE1 us with one, TILE16 with 16).
-    const int tile = static_cast<long>(a.n) * 2 * a.nkv <= 32768 ? 1 : 16;
-    const long groups = (a.slots != nullptr ? static_cast<long>(pl_ceil_div(a.n, tile)) * 2 * a.nkv : 0) + (static_cast<long>(a.n) * pl_ceil_div(a.nq, P8_HEADS) + ROWS - 1) / ROWS;
+    constexpr int ROWS = P8_WAVES * PL_WAVE / LPR;
+    // A wave takes a run, 64 / LPR rows at a time; in steps of many rows a workgroup does, four times as many.  It looks through `tile` rows for the first ones of runs: one each while all of a
+    // step's may be first (decoding), else 32, since most of many rows are inside a page, and units that find nothing still cost their start: 10,503 rows of prompts into 8 heads take 182 us with a
+    // workgroup a row and 77 with 32 rows, 600 single tokens 30 us with a workgroup each and 14 with a wave.  (Values of more rows held in registers, so that a run is not read again from L2 once its
+    // power is known, cost the queries' workgroups of the same launch their places: 94 us with twice the rows, 117 with four times.)
+    const int tile = static_cast<long>(a.n) * 2 * a.nkv <= P8_SINGLE_UNITS ? 1 : 32;
+    const bool whole = tile > 1 && a.block > PL_WAVE / LPR;
+    const long units = a.slots != nullptr ? static_cast<long>(pl_ceil_div(a.n, tile)) * 2 * a.nkv : 0;
+    const long groups = (whole ? units : (units + P8_WAVES - 1) / P8_WAVES) + (static_cast<long>(a.n) * pl_ceil_div(a.nq, P8_HEADS) + ROWS - 1) / ROWS;
     PL_REQUIRE(groups < (1l << 31) && static_cast<long>(a.n) * a.nq < (1l << 31) - ROWS, "8-bit write: %d rows of %d heads are too many for a launch", a.n, a.nq + 2 * a.nkv);
     const bool pieces = a.rot == 0 || (a.rot % 16 == 0 && !a.neighbours && (reinterpret_cast<uintptr_t>(a.cos) | reinterpret_cast<uintptr_t>(a.sin)) % 16 == 0);
-    if (pieces) write_8bit_kernel<T, LPR, WAVES, true><<<static_cast<unsigned>(groups), WAVES * PL_WAVE, 0, stream>>>(a, tile);
-    else write_8bit_kernel<T, LPR, WAVES, false><<<static_cast<unsigned>(groups), WAVES * PL_WAVE, 0, stream>>>(a, tile);
+    const auto kernel = whole ? (pieces ? write_8bit_kernel<T, LPR, P8_WAVES, true> : write_8bit_kernel<T, LPR, P8_WAVES, false>)
+                              : (pieces ? write_8bit_kernel<T, LPR, 1, true> : write_8bit_kernel<T, LPR, 1, false>);
+    kernel<<<static_cast<unsigned>(groups), P8_WAVES * PL_WAVE, 0, stream>>>(a, tile);
     PL_CHECK_LAUNCH("write_8bit");
     return 0;
 }
