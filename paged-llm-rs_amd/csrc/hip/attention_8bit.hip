@@ -2,7 +2,7 @@
 //
 //   out = softmax(scale q . k) v,   k = 2^Ek[page] e4m3,   v = 2^Ev[page] e4m3
 //
-// An e4m3 value times a power of two is exact in bfloat16, so keys and values become bfloat16 in one instruction for two of them
+// An e4m3 value times a power of two is exact in bfloat16 (but for the last sixteenth below the type's largest, which pages may have rounded up past it), so keys and values become bfloat16 in one instruction for two of them
 // (v_cvt_scalef32_pk_bf16_fp8) and both products run on the matrix cores' bfloat16 instruction with 32-bit sums.  Queries and weights in bfloat16 are one operand; in 32 bits a number is
 // three bfloat16 numbers (8 + 8 + 8 bits of it) whose products with the cache are exact, so the 32-bit path is three products of bfloat16 and not
 // one of the 32-bit instruction, which is sixteen times slower.
@@ -111,6 +111,8 @@ __device__ __forceinline__ bool a8_brings(const A8Args& a, int s) {
 template <int PIECES, int DQ>
 struct A8Few {
     static constexpr int BLOCKS = PIECES == 1 ? (DQ <= 2 ? 4 : 2) : (DQ == 1 ? 4 : DQ == 2 ? 2 : 1);
+    // waves a SIMD: two where 256 registers hold a wave's
+    static constexpr int WAVES(int blocks) { return PIECES * blocks * DQ > 6 || (DQ == 3 && blocks == 2) || (PIECES == 3 && blocks * DQ > 1) ? 1 : 2; }
 };
 
 // Which request and which of its blocks of rows is number `slot`, counted over the requests of more than `few` rows one after the other; by a whole wave.
@@ -171,9 +173,11 @@ __device__ __forceinline__ void a8_query8(const A8Args& a, size_t at, bool there
 // A workgroup takes the RB blocks of 16 rows of one request and key head and one share of the keys; its waves take tiles of 32 keys in turn, each with a running maximum and sum, and meet at the end.
 // Keys go from memory into the registers that the product reads (a lane reads 16 bytes of one key: the contraction may go through a head's values in any order, so the
 // queries are laid out to match); values go through a piece of LDS that belongs to the wave, so the loop has no barrier.  The next tile's bytes are on their way while a tile is worked on.
+// Bound by memory: 64 single tokens of 32 heads over 8 at contexts of 1,000 to 12,000 read 857 MB in 203 us, 4.2 TB/s (a copy of 4 GB moves 4.6, pieces of 128 bytes as these are read at 5.3), and their shares are
+// put together in another 7.  A wave has one key head: four heads' pieces side by side would be read at 6.2 TB/s, but with four times the shares to put together.
 //   S^T = K . Q^T: v_mfma_f32_16x16x32_bf16, twice for 32 keys; a lane has for row lane % 16 the keys 4 (lane / 16) .. + 3 of both.  DQ: the head is padded to 64 DQ values.
 template <int PIECES, int DQ, int RB>
-__global__ __launch_bounds__(A8_WAVES * PL_WAVE, PIECES * RB * DQ > 6 || (PIECES == 3 && RB * DQ > 1) ? 1 : 2) void attention_8bit_few_kernel(A8Args a) {
+__global__ __launch_bounds__(A8_WAVES * PL_WAVE, (A8Few<PIECES, DQ>::WAVES(RB))) void attention_8bit_few_kernel(A8Args a) {
     constexpr int DP = 64 * DQ, VROW = DP + 16;              // (16 more: eight rows read transposed fall on every bank once)
     constexpr int MROW = DP + 4;
     constexpr int VALUES = A8_WAVES * A8_KEYS * VROW * 2, MEET = 2 * 16 * MROW * 4;
@@ -435,9 +439,12 @@ __global__ __launch_bounds__(A8_WAVES * PL_WAVE, PIECES * RB * DQ > 6 || (PIECES
 // A workgroup takes NW blocks of 32 rows of one request and key head and one share of the keys, a block a wave.  Tiles of 32 KB keys come into LDS as bfloat16, so what an e4m3 value costs to widen is
 // paid once for all the rows.
 //   S^T = K . Q^T: v_mfma_f32_32x32x16_bf16; a lane has for row lane % 32 the keys 8 (i / 4) + 4 (lane / 32) + i % 4 of 32.  DT: the head is padded to 32 DT values.
-// What bounds it is the weights: an exponential takes a wave four times as long as another vector instruction, and together they take as long as the products.  So the scores of the next tile are multiplied while
-// the weights of this one are made, and the next maximum is found while this tile's weights meet its values: both pipes work in one wave, whatever the other waves of the unit do.
-// For that the keys in LDS are a tile ahead of the values (two lengths of keys, three of values), their bytes another tile ahead in registers, and their pages one more.  A round has one barrier.
+// What bounds it is what a SIMD can issue: of a tile of 64 keys and 128 values a wave's products take 1,024 cycles, its other vector instructions some 1,060 (an exponential as long as two of the rest), and LDS,
+// which every wave reads whole, another 500 a wave and its share of the unit.  So the scores of the next tile are multiplied while the weights of this one are made, and the next maximum is found while
+// this tile's weights meet its values: both pipes work in one wave, whatever the other wave of the SIMD does.  For that the keys in LDS are a tile ahead of the values (two lengths of keys, three of
+// values), their bytes another tile ahead in registers, and their pages one more.  A round has one barrier.  8,100 tokens of 32 heads over 8 take 0.53 ms, 1,010 TFLOP/s (a large matrix product of the library
+// reaches 1,450 on the same card); without the overlap 0.69.  Tried and slower: the two waves of a SIMD half a round apart with a barrier a half (0.64), 64 rows a wave with all 512 registers (0.85: moves
+// between the two halves of the register file).
 template <int PIECES, int DT>
 struct A8Many {
     static constexpr int KB = DT == 8 || (PIECES == 3 && DT != 4) ? 1 : 2;     // (what 160 KB of LDS hold; in 32 bits what leaves two waves a SIMD their registers, where that can be)
