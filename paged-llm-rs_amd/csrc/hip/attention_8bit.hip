@@ -169,6 +169,18 @@ __device__ __forceinline__ void a8_query8(const A8Args& a, size_t at, bool there
     }
 }
 
+// The maximum of a lane's number and that of lane ^ 32.
+__device__ __forceinline__ float a8_max_half(float v) {
+    const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1]));
+}
+// And of those of lanes ^ 16, ^ 32 and ^ 48.
+__device__ __forceinline__ float a8_max_quarters(float v) {
+    v = a8_max_half(v);
+    const auto both = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1]));
+}
+
 // ---- few rows: every wave has keys of its own ------------------------------------------------------------------------------
 // A workgroup takes the RB blocks of 16 rows of one request and key head and one share of the keys; its waves take tiles of 32 keys in turn, each with a running maximum and sum, and meet at the end.
 // Keys go from memory into the registers that the product reads (a lane reads 16 bytes of one key: the contraction may go through a head's values in any order, so the
@@ -346,8 +358,7 @@ __global__ __launch_bounds__(A8_WAVES * PL_WAVE, (A8Few<PIECES, DQ>::WAVES(RB)))
                 }
                 top = fmaxf(top, x[e]);
             }
-            top = fmaxf(top, __shfl_xor(top, 16, PL_WAVE));
-            top = fmaxf(top, __shfl_xor(top, 32, PL_WAVE));
+            top = a8_max_quarters(top);
             const float from = top == -INFINITY ? 0.f : top;
             const float alpha = __builtin_amdgcn_exp2f(m[b] - from);
             m[b] = top;
@@ -452,12 +463,6 @@ struct A8Many {
     static constexpr int KROW = 32 * DT + 8, VROW = 32 * DT + (DT % 2 == 0 ? 32 : 0);
     static constexpr size_t LDS = static_cast<size_t>(32 * KB) * (2 * KROW + 3 * VROW) * 2;
 };
-
-// The maximum of a lane's number and that of lane ^ 32.
-__device__ __forceinline__ float a8_max_half(float v) {
-    const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1]));
-}
 
 template <int PIECES, int DT, int NW>
 __global__ __launch_bounds__(NW * PL_WAVE) __attribute__((amdgpu_waves_per_eu(A8Many<PIECES, DT>::WAVES, A8Many<PIECES, DT>::WAVES))) void attention_8bit_many_kernel(A8Args a, int few) {
