@@ -3048,7 +3048,8 @@ def qk_norm_rope_kv_write_8bit(qkv: torch.Tensor, q: torch.Tensor | None, q_gain
 def shares_8bit(n: int, requests: int, max_ctx: int, nq: int, nkv: int, window: int = 0) -> tuple:
     """(keys a share, shares) of the 8-bit attention's kernel of few rows, and the same of its kernel of many.
 
-    Few rows: the longest shares, up to 2,048 keys, that still give the chip some 200 workgroups: every share costs a start of some 3 us and leaves a row of results to be put together.
+    Few rows: the longest shares, up to 2,048 keys, that still give the chip some 200 workgroups: every share costs a start of some 5 us and leaves a row of results to be put together (8 tokens at 4,000 keys: 20 us in
+    shares of 1,024, 25 in 256 or 2,048).  Contexts of up to 640 keys stay whole, which saves the launch that puts shares together (8 tokens at 300 keys: 7.9 us instead of 9.5, at 640 9.8 and 10.8, at 800 11.6 and 10.2).
     Many rows: as many shares as still leave every workgroup a compute unit of its own, none of fewer than 256 keys.  A share writes and reads its rows' outputs in 32 bits, and two workgroups
     on a unit are no faster than one after the other: 2,048 fresh tokens of 32 heads take 65 us in their 256 blocks and 87 with the keys cut in two, 512 tokens behind 15,500 (64 blocks) 384 us whole, 144 in four, 156 in eight."""
     def of(chunk, reach):
@@ -3058,7 +3059,7 @@ def shares_8bit(n: int, requests: int, max_ctx: int, nq: int, nkv: int, window: 
 
     reach = min(max_ctx, abs(window) + 64) if window else max_ctx
     chunk = 2048
-    while chunk > 128 and requests * nkv * ((reach + chunk - 1) // chunk) < 200:
+    while max_ctx > 640 and chunk > 128 and requests * nkv * ((reach + chunk - 1) // chunk) < 200:
         chunk //= 2
     few = of(min(chunk, (max_ctx + 31) // 32 * 32), reach)
     reach = min(max_ctx, abs(window) + 256) if window else max_ctx

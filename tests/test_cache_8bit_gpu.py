@@ -556,10 +556,10 @@ def test_pages_behind_four_gigabytes():
     near = scene.pages
     scene.pages, scene.table = far, table
     assert torch.equal(scene.run(), want)
-    qkv = torch.randn(40, 3 * 8 * 128, device=DEV).to(torch.bfloat16)
+    qkv = torch.randn(40, (4 + 2 * 8) * 128, device=DEV).to(torch.bfloat16)
     slots = i32([3 * 16 + 5 + i for i in range(40)])
-    write(near, qkv, slots, i32(list(range(40))), 8)
-    write(far, qkv, slots + (total - few) * 16, i32(list(range(40))), 8)
+    write(near, qkv, slots, i32(list(range(40))), 4)
+    write(far, qkv, slots + (total - few) * 16, i32(list(range(40))), 4)
     for big, small in zip(far, near):
         assert torch.equal(big.view(torch.uint8)[-small.shape[0]:], small.view(torch.uint8))
     made = kernels.step_tables(scene.q_len, scene.ctx_len, table, 16, None, scene.n)
