@@ -49,6 +49,7 @@ struct A8Args {
     int shift, pages;
     const uint8_t *k_pool, *v_pool, *k_scale, *v_scale;
     int nq, nkv, d;
+    int beside;               // key heads whose rows share lines of memory (a8_beside)
     float scale;              // times log2(e)
     int window;
     int n, chunk, chunks;     // rows of the step; keys a workgroup, and how many such shares the longest context has
@@ -114,6 +115,26 @@ struct A8Few {
     // waves a SIMD: two where 256 registers hold a wave's
     static constexpr int WAVES(int blocks) { return PIECES * blocks * DQ > 6 || (DQ == 3 && blocks == 2) || (PIECES == 3 && blocks * DQ > 1) ? 1 : 2; }
 };
+
+// Workgroups go to the chip's eight XCDs in turn, and each XCD has an L2 of its own: where a line of 128 bytes holds several key heads' values, those heads' workgroups (`beside` of them) are dealt to one
+// XCD, one turn behind the other, so the line is read from memory once (16 tokens at 4,000 keys, 8 key heads of 64: 27 us with neighbours on eight XCDs, 21 with them on one; 12 heads of 96: 55 and 38).
+// Number `block` of a grid of a8_grid(...) is a unit (a request, or a block of rows), a key head and a share of the keys; false: there is no such unit.
+#define A8_XCDS 8
+__device__ __forceinline__ bool a8_deal(const A8Args& a, int block, int units, int& unit, int& kvh, int& share) {
+    const int groups = a.nkv / a.beside, turn = block / A8_XCDS;
+    const int at = turn / a.beside * A8_XCDS + block % A8_XCDS, rest = at / groups;
+    kvh = at % groups * a.beside + turn % a.beside;
+    share = rest / units;
+    unit = rest - share * units;
+    return share < a.chunks;
+}
+static long a8_grid(const A8Args& a, long units) { return (units * a.chunks * (a.nkv / a.beside) + A8_XCDS - 1) / A8_XCDS * A8_XCDS * a.beside; }
+// The fewest heads (at most eight, that divide their number) that fill whole lines together.
+static int a8_beside(int nkv, int d) {
+    int heads = 1;
+    while (heads < 8 && heads * d % 128 != 0 && nkv % (2 * heads) == 0) heads *= 2;
+    return heads;
+}
 
 // Which request and which of its blocks of rows is number `slot`, counted over the requests of more than `few` rows one after the other; by a whole wave.
 __device__ __forceinline__ bool a8_find(const A8Args& a, int slot, int group, int rows, int few, int& seq, int& block) {
@@ -203,11 +224,11 @@ __global__ __launch_bounds__(A8_WAVES * PL_WAVE, (A8Few<PIECES, DQ>::WAVES(RB)))
     const int tid = threadIdx.x, lane = tid % PL_WAVE, wave = tid / PL_WAVE;
     const int col = lane % 16, quarter = lane / 16;
     const int group = a.nq / a.nkv;
-    const int kvh = blockIdx.x % a.nkv, seq = blockIdx.x / a.nkv;
-    if (!a8_brings(a, seq) || a.q_len[seq] * group > 16 * RB) return;
+    int kvh, seq, share;
+    if (!a8_deal(a, blockIdx.x, a.S, seq, kvh, share) || !a8_brings(a, seq) || a.q_len[seq] * group > 16 * RB) return;
     const int q_len = a.q_len[seq], start = a.ctx_len[seq] - q_len, rows = q_len * group;
     const int lo = pl_first_visible(start, a.window), hi = start + q_len;
-    const int shares = a8_shares(lo, hi, a.chunk), share = blockIdx.y;
+    const int shares = a8_shares(lo, hi, a.chunk);
     if (share >= shares) return;
     const int k_base = (lo / a.chunk + share) * a.chunk;
     const int k_begin = max(lo, k_base), k_end = min(hi, k_base + a.chunk);
@@ -465,7 +486,7 @@ struct A8Many {
 };
 
 template <int PIECES, int DT, int NW>
-__global__ __launch_bounds__(NW * PL_WAVE) __attribute__((amdgpu_waves_per_eu(A8Many<PIECES, DT>::WAVES, A8Many<PIECES, DT>::WAVES))) void attention_8bit_many_kernel(A8Args a, int few) {
+__global__ __launch_bounds__(NW * PL_WAVE) __attribute__((amdgpu_waves_per_eu(A8Many<PIECES, DT>::WAVES, A8Many<PIECES, DT>::WAVES))) void attention_8bit_many_kernel(A8Args a, int few, int units) {
     constexpr int KB = A8Many<PIECES, DT>::KB, TILE = 32 * KB, KROW = A8Many<PIECES, DT>::KROW, VROW = A8Many<PIECES, DT>::VROW, THREADS = NW * PL_WAVE;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     uint16_t* keys = reinterpret_cast<uint16_t*>(lds);                 // [2][TILE][KROW]
@@ -474,13 +495,12 @@ __global__ __launch_bounds__(NW * PL_WAVE) __attribute__((amdgpu_waves_per_eu(A8
     const int tid = threadIdx.x, lane = tid % PL_WAVE, wave = __builtin_amdgcn_readfirstlane(tid / PL_WAVE);
     const int col = lane % 32, half = lane / 32;
     const int group = a.nq / a.nkv;
-    const int kvh = blockIdx.x % a.nkv;
-    int seq, rb;
-    if (!a8_find(a, blockIdx.x / a.nkv, group, 32 * NW, few, seq, rb)) return;
+    int kvh, unit, share, seq, rb;
+    if (!a8_deal(a, blockIdx.x, units, unit, kvh, share) || !a8_find(a, unit, group, 32 * NW, few, seq, rb)) return;
     const int q_len = a.q_len[seq], start = a.ctx_len[seq] - q_len, q_start = a.q_start[seq];
     const int first_row = rb * 32 * NW, rows = min(32 * NW, q_len * group - first_row);
     const int lo = pl_first_visible(start + first_row / group, a.window), hi = start + (first_row + rows - 1) / group + 1;
-    const int shares = a8_shares(lo, hi, a.chunk), share = blockIdx.y;
+    const int shares = a8_shares(lo, hi, a.chunk);
     if (share >= shares) return;
     const int k_base = (lo / a.chunk + share) * a.chunk;
     const int k_begin = max(lo, k_base), k_end = min(hi, k_base + a.chunk);
@@ -789,10 +809,11 @@ static int a8_lds(const void* kernel, size_t lds) {
 
 template <int PIECES, int DQ, int RB>
 static int launch_few(const A8Args& a, int rows, hipStream_t stream) {
+    PL_REQUIRE(a8_grid(a, a.S) < (1l << 31), "8-bit attention: %d requests in %d shares are too many for a launch", a.S, a.chunks);
     const size_t lds = static_cast<size_t>(A8_WAVES) * A8_KEYS * (64 * DQ + 16) * 2 + A8_WAVES * 2 * 16 * RB * 4 + static_cast<size_t>(a.chunk) * 6;
     if (int e = a8_lds(reinterpret_cast<const void*>(&attention_8bit_few_kernel<PIECES, DQ, RB>), lds)) return e;
     const unsigned blocks = static_cast<unsigned>(a.S) * a.nkv;
-    attention_8bit_few_kernel<PIECES, DQ, RB><<<dim3(blocks, a.chunks), A8_WAVES * PL_WAVE, lds, stream>>>(a);
+    attention_8bit_few_kernel<PIECES, DQ, RB><<<static_cast<unsigned>(a8_grid(a, a.S)), A8_WAVES * PL_WAVE, lds, stream>>>(a);
     PL_CHECK_LAUNCH("attention_8bit_few");
     if (a.chunks > 1) {
         attention_8bit_merge_kernel<typename A8Type<PIECES>::type><<<dim3(blocks, pl_ceil_div(rows, A8_WAVES)), A8_WAVES * PL_WAVE, 0, stream>>>(a, 16 * RB, 0);
@@ -828,8 +849,8 @@ template <int PIECES, int DT, int NW>
 static int launch_many(const A8Args& a, int few, long blocks, hipStream_t stream) {
     const size_t lds = A8Many<PIECES, DT>::LDS;
     if (int e = a8_lds(reinterpret_cast<const void*>(&attention_8bit_many_kernel<PIECES, DT, NW>), lds)) return e;
-    PL_REQUIRE(blocks * a.nkv < (1l << 31), "8-bit attention: %ld blocks of rows are too many for a launch", blocks);
-    attention_8bit_many_kernel<PIECES, DT, NW><<<dim3(static_cast<unsigned>(blocks * a.nkv), a.chunks), NW * PL_WAVE, lds, stream>>>(a, few);
+    PL_REQUIRE(a8_grid(a, blocks) < (1l << 31), "8-bit attention: %ld blocks of rows in %d shares are too many for a launch", blocks, a.chunks);
+    attention_8bit_many_kernel<PIECES, DT, NW><<<static_cast<unsigned>(a8_grid(a, blocks)), NW * PL_WAVE, lds, stream>>>(a, few, static_cast<int>(blocks));
     PL_CHECK_LAUNCH("attention_8bit_many");
     if (a.chunks > 1) {
         attention_8bit_merge_kernel<typename A8Type<PIECES>::type><<<dim3(static_cast<unsigned>(blocks * a.nkv), 4 * NW), A8_WAVES * PL_WAVE, 0, stream>>>(a, few, 32 * NW);
@@ -876,7 +897,7 @@ extern "C" int pl_paged_attention_8bit(const void* q, int q_stride, void* out, c
     PL_REQUIRE(nkv >= 1 && nq >= nkv && nq % nkv == 0, "8-bit attention: %d query heads over %d key heads", nq, nkv);
     PL_REQUIRE(S >= 1 && n >= 1 && max_q_len >= 1 && min_q_len <= max_q_len && width >= 1 && block >= 1 && pool_rows >= block,
                "8-bit attention: %d requests, %d rows, %d to %d of one request, tables of %d pages of %d, %d rows", S, n, min_q_len, max_q_len, width, block, pool_rows);
-    PL_REQUIRE(static_cast<long>(n) * nq < (1l << 31) && static_cast<long>(S) * nkv < (1l << 31), "8-bit attention: %d rows of %d heads, %d requests are too many for a launch", n, nq, S);
+    PL_REQUIRE(static_cast<long>(n) * nq < (1l << 31) && (static_cast<long>(S) + 8) * nkv < (1l << 31), "8-bit attention: %d rows of %d heads, %d requests are too many for a launch", n, nq, S);
     PL_REQUIRE(few_chunk >= A8_KEYS && few_chunk % A8_KEYS == 0 && few_chunk <= A8_MOST_KEYS && few_chunks >= 1 && few_chunks < 65536 && (few_chunks == 1 || (part_acc && part_ml)),
                "8-bit attention: %d shares of %d keys", few_chunks, few_chunk);
     PL_REQUIRE(many_chunk >= 64 && many_chunk % 64 == 0 && many_chunks >= 1 && many_chunks < 65536 && (many_chunks == 1 || (part_acc && part_ml)),
@@ -885,7 +906,7 @@ extern "C" int pl_paged_attention_8bit(const void* q, int q_stride, void* out, c
     const uint32_t magic = static_cast<uint32_t>(((uint64_t{1} << shift) + block - 1) / block);
     A8Args a{q, q_stride, out, static_cast<const int*>(q_start), static_cast<const int*>(q_len), static_cast<const int*>(ctx_len), S, static_cast<const int*>(table), width, block, magic, shift, pool_rows / block,
              static_cast<const uint8_t*>(k_pool), static_cast<const uint8_t*>(v_pool), static_cast<const uint8_t*>(k_scale), static_cast<const uint8_t*>(v_scale),
-             nq, nkv, d, scale * 1.4426950408889634f, window, n, few_chunk, few_chunks, static_cast<float*>(part_acc), static_cast<float*>(part_ml)};
+             nq, nkv, d, a8_beside(nkv, d), scale * 1.4426950408889634f, window, n, few_chunk, few_chunks, static_cast<float*>(part_acc), static_cast<float*>(part_ml)};
     const long group = nq / nkv, longest = max_q_len * group;
     // In a step of portions only what 16 rows hold goes to the kernel of few: those are the single tokens beside them, for which its smallest form is the fastest
     // (15 single tokens at up to 4,600 keys beside a portion: 32 us with it, 91 with the form for 64 rows).
