@@ -859,13 +859,23 @@ static int launch_many(const A8Args& a, int few, long blocks, hipStream_t stream
     return 0;
 }
 
-template <int PIECES, int DT>
-static int launch_many(const A8Args& a, int few, int max_q_len, hipStream_t stream) {
-    constexpr int NW = PIECES * DT >= 6 ? 4 : 8;
+template <int PIECES, int DT, int NW>
+static int launch_many_blocks(const A8Args& a, int few, int max_q_len, hipStream_t stream) {
     const int group = a.nq / a.nkv;
     // blocks of rows: one a request for what is left over, and the whole ones
     const long most = static_cast<long>(a.S) * ((static_cast<long>(max_q_len) * group + 32 * NW - 1) / (32 * NW)), all = a.S + static_cast<long>(a.n) * group / (32 * NW);
     return launch_many<PIECES, DT, NW>(a, few, most < all ? most : all, stream);
+}
+
+// Four waves a workgroup where eight's registers or LDS leave no second one beside it anyway (32 bits, heads of more than 128) or where two of four fit a unit (heads of up to 64: 2 prompts of 1,500 to 2,000 tokens,
+// 16 heads over 8, 45 us with eight, 40 with four); else eight, which widen a tile for 256 rows, but for so few rows that workgroups of 128 do not fill the chip either (512 tokens of 16 heads over 8: 23.5 and 20.8 us).
+template <int PIECES, int DT>
+static int launch_many(const A8Args& a, int few, int max_q_len, hipStream_t stream) {
+    if constexpr (PIECES == 1 && (DT == 3 || DT == 4)) {
+        const long blocks = (static_cast<long>(a.n) * (a.nq / a.nkv) + 127) / 128 * a.nkv * a.chunks;
+        if (blocks > 256) return launch_many_blocks<PIECES, DT, 8>(a, few, max_q_len, stream);
+    }
+    return launch_many_blocks<PIECES, DT, 4>(a, few, max_q_len, stream);
 }
 
 template <int PIECES>
