@@ -3015,7 +3015,7 @@ def qk_norm_rope_kv_write_8bit(qkv: torch.Tensor, q: torch.Tensor | None, q_gain
     What is not finite is kept as NaN.
 
     The rows that go into one page follow each other with slots that follow each other, as those of a request's tokens do, and no page is named twice; a slot below 0 (or past the
-    pool) is written nowhere, and the queries of a row with a position below 0 are left as they were.  ``write_kv=False``: the queries alone."""
+    pool) is written nowhere, and the queries of a row with a position below 0 are left as they were; a position past the rotary tables takes their last row.  ``write_kv=False``: the queries alone."""
     device = torch.cuda.current_device()
     code = _code(qkv, "fused q/k/v projection")
     rows, keys, values, key_powers, value_powers = _pages_8bit(k_pool, v_pool, k_scale, v_scale, block_size, nkv, d, device)
@@ -3040,7 +3040,7 @@ def qk_norm_rope_kv_write_8bit(qkv: torch.Tensor, q: torch.Tensor | None, q_gain
         raise TensorError("rows and gains for an 8-bit cache begin at whole 16 bytes")
     places = _fits(slots, "slots", torch.int32, n, device) if write_kv else 0
     _check(library().pl_qk_norm_rope_kv_write_8bit(
-        source, queries, stride, q_gains, k_gains, gain_code, eps, cosines, sines, rot, angles, 1 if neighbours else 0, _fits(positions, "positions", torch.int32, n, device), places,
+        source, queries, stride, q_gains, k_gains, gain_code, float(eps), cosines, sines, rot, angles, 1 if neighbours else 0, _fits(positions, "positions", torch.int32, n, device), places,
         block_size, rows, keys, values, key_powers, value_powers, n, nq, nkv, d, code, _stream_of(device)))
 
 
@@ -3076,8 +3076,10 @@ def paged_attention_8bit(q: torch.Tensor, q_row_stride: int, out: torch.Tensor, 
     as they were in ``out``.
 
     ``max_q_len``, ``min_q_len`` and ``max_ctx`` bound what the requests bring and their contexts (the launches are sized and chosen by them): rows whose keys reach past ``max_ctx`` come out as NaN, and
-    rows past ``max_q_len`` of a request may be left out.  The caller answers for the pages of all keys that are seen; keys that no row of a request sees may hold anything."""
+    rows past ``max_q_len`` of a request may be left out.  The caller answers for the pages of all keys that are seen; keys that no row of a request sees may hold anything
+    (a NaN among the values that some row sees may reach the other rows that its request brings)."""
     device = torch.cuda.current_device()
+    max_q_len, min_q_len, max_ctx, window = int(max_q_len), int(min_q_len), int(max_ctx), int(window or 0)
     code = _code(q, "query buffer")
     if nkv < 1 or nq < 1 or nq % nkv:
         raise TensorError(f"{nq} query heads over {nkv} key heads, which do not group evenly")
@@ -3095,7 +3097,6 @@ def paged_attention_8bit(q: torch.Tensor, q_row_stride: int, out: torch.Tensor, 
     queries, results = _fits(q, "query buffer", q.dtype, n * q_row_stride, device), _fits(out, "attention output", q.dtype, n * nq * d, device, (n, nq * d))
     if q_row_stride % 8 or (queries | results) % 16:
         raise TensorError("query rows and outputs for an 8-bit cache begin at whole 16 bytes")
-    window = int(window or 0)
     few, few_shares, many, many_shares = shares_8bit(n, S, max_ctx, nq, nkv, window)
     chunks = max(few_shares, many_shares)
     acc = ml = 0
@@ -3106,7 +3107,7 @@ def paged_attention_8bit(q: torch.Tensor, q_row_stride: int, out: torch.Tensor, 
     _check(library().pl_paged_attention_8bit(
         queries, q_row_stride, results, _fits(q_start, "first row of each request", torch.int32, S, device), _fits(q_len, "tokens of each request", torch.int32, S, device),
         _fits(ctx_len, "context length of each request", torch.int32, S, device), S, n, max_q_len, min_q_len, _fits(block_table, "block table", torch.int32, S * width, device), width,
-        block_size, rows, keys, values, key_powers, value_powers, nq, nkv, d, scale, window, few, few_shares, many, many_shares, acc, ml, code, _stream_of(device)))
+        block_size, rows, keys, values, key_powers, value_powers, nq, nkv, d, float(scale), window, few, few_shares, many, many_shares, acc, ml, code, _stream_of(device)))
     return out
 
 
