@@ -28,7 +28,8 @@ typedef __attribute__((address_space(3))) a8_bf16x4 a8_lds_bf16x4;
 
 #define A8_KEYS 32       // keys a wave's tile where every wave has keys of its own
 #define A8_WAVES 4
-#define A8_MOST_KEYS 2048   // of a share of few rows
+#define A8_MOST_KEYS 2048   // of a share of few rows as the caller cuts them, and as the kernel itself may (a8_balance):
+#define A8_MOST_BALANCED 4096
 
 union a8_frag {
     a8_bf16x8 vec;
@@ -53,6 +54,7 @@ struct A8Args {
     float scale;              // times log2(e)
     int window;
     int n, chunk, chunks;     // rows of the step; keys a workgroup, and how many such shares the longest context has
+    int most, places;         // few rows: the most keys a workgroup, and how many workgroups the chip holds at once (a8_balance)
     float *part_acc, *part_ml;
 };
 
@@ -102,6 +104,9 @@ __device__ __forceinline__ void a8_split(const float (&x)[8], a8_frag (&to)[PIEC
     }
 }
 
+// Whether keys are more than the caller's longest context has.
+__device__ __forceinline__ bool a8_late(const A8Args& a, int keys) { return keys > static_cast<long>(a.chunk) * a.chunks; }
+
 // Whether request s brings rows.  (One whose context is shorter than what it brings holds the rows of a padded step.)
 __device__ __forceinline__ bool a8_brings(const A8Args& a, int s) {
     const int q = a.q_len[s], c = a.ctx_len[s], at = a.q_start[s];         // (all three at once)
@@ -128,12 +133,59 @@ __device__ __forceinline__ bool a8_deal(const A8Args& a, int block, int units, i
     unit = rest - share * units;
     return share < a.chunks;
 }
-static long a8_grid(const A8Args& a, long units) { return (units * a.chunks * (a.nkv / a.beside) + A8_XCDS - 1) / A8_XCDS * A8_XCDS * a.beside; }
+static long a8_grid(const A8Args& a, long units, int chunks) { return (units * chunks * (a.nkv / a.beside) + A8_XCDS - 1) / A8_XCDS * A8_XCDS * a.beside; }
 // The fewest heads (at most eight, that divide their number) that fill whole lines together.
 static int a8_beside(int nkv, int d) {
     int heads = 1;
     while (heads < 8 && heads * d % 128 != 0 && nkv % (2 * heads) == 0) heads *= 2;
     return heads;
+}
+
+// Inclusive sums over a wave: within rows of 16 lanes, then the rows before.  (In the registers: a shuffle through LDS is some 50 ns a step.)
+__device__ __forceinline__ int a8_scan(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);         // from one lane below, two, four, eight
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);         // the last of a row to the row behind it (the second and the fourth)
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);         // the last of the first half to the second half
+    return v;
+}
+
+// Few rows of up to 64 requests whose shares are more than the chip holds at once: shares are made as much longer as brings them into the fewest rounds of the chip (a few workgroups in a round of their own take as
+// long as all those of a full one), and a request's are equally long.  By a whole wave; lane s says what request s has (its first key, its keys, its shares, the keys of one).  No two shares stand under one number, and numbers have no
+// gaps: workgroups without work between the others leave the shader engines, to which they go in turn, with more than they hold.
+// 8 requests of 40 rows at 9,000 to 24,000 keys, 64 heads over 8: 70 us, 97 in shares of 2,048; single tokens of 32 heads over 8: 32 at 1,500 to 8,000 keys 74 and 87, 16 at 1,500 to 16,000 66 and 70.
+struct A8Cut {
+    int start, q_len, q_start, lo, keys, shares, size;
+};
+__device__ __forceinline__ A8Cut a8_balance(const A8Args& a, int group, int few) {
+    const int s = threadIdx.x % PL_WAVE;
+    A8Cut cut{0, 0, 0, 0, 0, 0, 0};
+    if (s < a.S && a8_brings(a, s) && a.q_len[s] * group <= few) {
+        cut.q_len = a.q_len[s];
+        cut.q_start = a.q_start[s];
+        cut.start = a.ctx_len[s] - cut.q_len;
+        cut.lo = pl_first_visible(cut.start, a.window);
+        // (of a context longer than the caller said so much as there is room for: its outputs become NaN)
+        cut.keys = static_cast<int>(min(static_cast<long>(cut.start + cut.q_len - cut.lo), static_cast<long>(a.chunk) * a.chunks));
+    }
+    auto shares = [&](int size) { return cut.keys > 0 ? (cut.keys - 1) / size + 1 : 0; };
+    auto all = [&](int size) { return __builtin_amdgcn_readlane(a8_scan(shares(size)), PL_WAVE - 1) * a.nkv; };
+    int size = a.chunk;
+    if (all(size) > a.places) {
+        const int room = pl_ceil_div(all(a.most), a.places) * a.places;
+        int low = size / A8_KEYS, high = a.most / A8_KEYS;
+        while (low < high) {
+            const int mid = (low + high) / 2;
+            if (all(mid * A8_KEYS) <= room) high = mid;
+            else low = mid + 1;
+        }
+        size = high * A8_KEYS;
+    }
+    cut.shares = shares(size);
+    cut.size = cut.shares == 0 ? size : ((cut.keys - 1) / cut.shares / A8_KEYS + 1) * A8_KEYS;
+    return cut;
 }
 
 // Which request and which of its blocks of rows is number `slot`, counted over the requests of more than `few` rows one after the other; by a whole wave.
@@ -143,21 +195,16 @@ __device__ __forceinline__ bool a8_find(const A8Args& a, int slot, int group, in
         const int s = base + lane;
         int blocks = 0;
         if (s < a.S && a8_brings(a, s) && a.q_len[s] * group > few) blocks = pl_ceil_div(a.q_len[s] * group, rows);
-        int end = blocks;
-#pragma unroll
-        for (int off = 1; off < PL_WAVE; off <<= 1) {
-            const int up = __shfl_up(end, off, PL_WAVE);
-            if (lane >= off) end += up;
-        }
+        const int end = a8_scan(blocks);
         const uint64_t past = __ballot(end > slot);
         if (past != 0) {
             const int first = __ffsll(static_cast<unsigned long long>(past)) - 1;
             seq = __builtin_amdgcn_readfirstlane(base + first);
             // (the last rows, which see the most keys, first)
-            block = __builtin_amdgcn_readfirstlane(__shfl(end, first, PL_WAVE) - 1 - slot);
+            block = __builtin_amdgcn_readlane(end, first) - 1 - slot;
             return true;
         }
-        slot -= __shfl(end, PL_WAVE - 1, PL_WAVE);
+        slot -= __builtin_amdgcn_readlane(end, PL_WAVE - 1);
     }
     return false;
 }
@@ -209,7 +256,8 @@ __device__ __forceinline__ float a8_max_quarters(float v) {
 // Bound by memory: 64 single tokens of 32 heads over 8 at contexts of 1,000 to 12,000 read 857 MB in 203 us, 4.2 TB/s (a copy of 4 GB moves 4.6, pieces of 128 bytes as these are read at 5.3), and their shares are
 // put together in another 7.  A wave has one key head: four heads' pieces side by side would be read at 6.2 TB/s, but with four times the shares to put together.
 //   S^T = K . Q^T: v_mfma_f32_16x16x32_bf16, twice for 32 keys; a lane has for row lane % 16 the keys 4 (lane / 16) .. + 3 of both.  DQ: the head is padded to 64 DQ values.
-template <int PIECES, int DQ, int RB>
+//   BALANCED: with the shares of a8_balance.  (A build of its own: the one for shares as the caller cut them loses 0.4 to 1 us of 12 to 20 to what is only compiled in.)
+template <int PIECES, int DQ, int RB, bool BALANCED>
 __global__ __launch_bounds__(A8_WAVES * PL_WAVE, (A8Few<PIECES, DQ>::WAVES(RB))) void attention_8bit_few_kernel(A8Args a) {
     constexpr int DP = 64 * DQ, VROW = DP + 16;              // (16 more: eight rows read transposed fall on every bank once)
     constexpr int MROW = DP + 4;
@@ -219,25 +267,49 @@ __global__ __launch_bounds__(A8_WAVES * PL_WAVE, (A8Few<PIECES, DQ>::WAVES(RB)))
     uint16_t* values = reinterpret_cast<uint16_t*>(lds);
     float* stats = reinterpret_cast<float*>(lds + VALUES);   // [waves][2][rows]
     int* slots = reinterpret_cast<int*>(stats + A8_WAVES * 2 * 16 * RB);
-    uint16_t* units = reinterpret_cast<uint16_t*>(slots + a.chunk);          // (the two powers of a key, a byte each)
+    uint16_t* units = reinterpret_cast<uint16_t*>(slots + (BALANCED ? a.most : a.chunk));           // (the two powers of a key, a byte each)
 
     const int tid = threadIdx.x, lane = tid % PL_WAVE, wave = tid / PL_WAVE;
     const int col = lane % 16, quarter = lane / 16;
     const int group = a.nq / a.nkv;
-    int kvh, seq, share;
-    if (!a8_deal(a, blockIdx.x, a.S, seq, kvh, share) || !a8_brings(a, seq) || a.q_len[seq] * group > 16 * RB) return;
-    const int q_len = a.q_len[seq], start = a.ctx_len[seq] - q_len, rows = q_len * group;
-    const int lo = pl_first_visible(start, a.window), hi = start + q_len;
-    const int shares = a8_shares(lo, hi, a.chunk);
-    if (share >= shares) return;
-    const int k_base = (lo / a.chunk + share) * a.chunk;
-    const int k_begin = max(lo, k_base), k_end = min(hi, k_base + a.chunk);
+    int kvh, seq, share, q_len, q_start, start, lo, hi, shares, size, k_base;
+    if (!a8_deal(a, blockIdx.x, a.S, seq, kvh, share)) return;
+    if constexpr (BALANCED) {
+        const A8Cut cut = a8_balance(a, group, 16 * RB);
+        const int number = share * a.S + seq, end = a8_scan(cut.shares);
+        const uint64_t past = __ballot(end > number);
+        if (past == 0) return;
+        seq = __ffsll(static_cast<unsigned long long>(past)) - 1;
+        q_len = __builtin_amdgcn_readlane(cut.q_len, seq);
+        q_start = __builtin_amdgcn_readlane(cut.q_start, seq);
+        start = __builtin_amdgcn_readlane(cut.start, seq);
+        lo = __builtin_amdgcn_readlane(cut.lo, seq);
+        shares = __builtin_amdgcn_readlane(cut.shares, seq);
+        size = __builtin_amdgcn_readlane(cut.size, seq);
+        share = number - (__builtin_amdgcn_readlane(end, seq) - shares);
+        hi = start + q_len;
+        k_base = lo + share * size;
+        if (a8_late(a, hi - lo)) shares = a.chunks + 1;
+    } else {
+        if (!a8_brings(a, seq) || a.q_len[seq] * group > 16 * RB) return;
+        q_len = a.q_len[seq];
+        q_start = a.q_start[seq];
+        start = a.ctx_len[seq] - q_len;
+        lo = pl_first_visible(start, a.window);
+        hi = start + q_len;
+        size = a.chunk;
+        shares = a8_shares(lo, hi, size);
+        if (share >= shares) return;
+        k_base = (lo / size + share) * size;
+    }
+    const int rows = q_len * group;
+    const int k_begin = max(lo, k_base), k_end = k_base + min(hi - k_base, size);
     const int last_from = pl_first_visible(start + q_len - 1, a.window);     // (the last token's first key: no token's is later)
 
     // Where the keys of the share are, and in what units.  (Keys that no row sees are read at the nearest one's place.)  All pages are asked for, then all powers: one behind the other they would be a
     // wait each for every 256 keys.
-    constexpr int EACH = A8_MOST_KEYS / (A8_WAVES * PL_WAVE);
-    const int keys = min(pl_ceil_div(k_end - k_base, A8_KEYS) * A8_KEYS, a.chunk);
+    constexpr int EACH = (BALANCED ? A8_MOST_BALANCED : A8_MOST_KEYS) / (A8_WAVES * PL_WAVE);
+    const int keys = min(pl_ceil_div(k_end - k_base, A8_KEYS) * A8_KEYS, size);
     int page[EACH];
     const int* row_table = a.table + static_cast<size_t>(seq) * a.width;
 #pragma unroll
@@ -266,7 +338,6 @@ __global__ __launch_bounds__(A8_WAVES * PL_WAVE, (A8Few<PIECES, DQ>::WAVES(RB)))
     }
 
     // The rows: what a lane reads of a key with its j-th load are the values 64 j + 16 quarter .. + 15, two operands
-    const int q_start = a.q_start[seq];
     int seen_from[RB], seen[RB], out_row[RB];        // the keys of the share that a row sees: the first and how many
     a8_frag qf[RB][2 * DQ][PIECES];
 #pragma unroll
@@ -409,6 +480,7 @@ __global__ __launch_bounds__(A8_WAVES * PL_WAVE, (A8Few<PIECES, DQ>::WAVES(RB)))
         __builtin_amdgcn_wave_barrier();
     }
 
+    const bool whole_row = BALANCED ? shares == 1 : a.chunks == 1;       // (nothing to be put together)
     // The waves meet: maximum and sum first, then the outputs in halves, always in the same order.
 #pragma unroll
     for (int b = 0; b < RB; ++b) {
@@ -446,8 +518,8 @@ __global__ __launch_bounds__(A8_WAVES * PL_WAVE, (A8Few<PIECES, DQ>::WAVES(RB)))
         }
         if (wave == 0 && out_row[b] >= 0) {
             const size_t place = static_cast<size_t>(out_row[b]) * a.chunks + share;
-            if (a.chunks == 1) {
-                if (shares > 1) total = NAN;          // (a context longer than the caller said)
+            if (whole_row) {
+                if (!BALANCED && shares > 1) total = NAN;          // (a context longer than the caller said)
                 const float inv = total != 0.f ? 1.f / total : 0.f;
 #pragma unroll
                 for (int t = 0; t < 4 * DQ; ++t) acc[b][t] *= inv;
@@ -460,7 +532,7 @@ __global__ __launch_bounds__(A8_WAVES * PL_WAVE, (A8Few<PIECES, DQ>::WAVES(RB)))
                 const int c = 16 * t + 4 * quarter;           // (as the values stood in LDS)
                 const int at = 16 * (c % (DP / 2) / 8) + 8 * (c / (DP / 2)) + c % 8;
                 if (at >= a.d) continue;
-                if (a.chunks == 1) a8_store4<PIECES>(a, static_cast<size_t>(out_row[b]) * a.d + at, acc[b][t][0], acc[b][t][1], acc[b][t][2], acc[b][t][3]);
+                if (whole_row) a8_store4<PIECES>(a, static_cast<size_t>(out_row[b]) * a.d + at, acc[b][t][0], acc[b][t][1], acc[b][t][2], acc[b][t][3]);
                 else *reinterpret_cast<a8_f32x4*>(a.part_acc + place * a.d + at) = acc[b][t];
             }
         }
@@ -758,7 +830,13 @@ __global__ __launch_bounds__(A8_WAVES * PL_WAVE) void attention_8bit_merge_kerne
     const int q_len = a.q_len[seq], start = a.ctx_len[seq] - q_len;
     const int first_row = rb * per, rows = min(per > 0 ? per : few, q_len * group - first_row);
     const int lo = pl_first_visible(start + first_row / group, a.window), hi = start + (first_row + rows - 1) / group + 1;
-    const int all = a8_shares(lo, hi, a.chunk), shares = min(all, a.chunks);
+    int all = a8_shares(lo, hi, a.chunk);
+    if (per == 0 && a.most > a.chunk) {
+        const A8Cut cut = a8_balance(a, group, few);
+        all = a8_late(a, hi - lo) ? a.chunks + 1 : __builtin_amdgcn_readlane(cut.shares, seq);
+        if (all == 1) return;             // (written as they are)
+    }
+    const int shares = min(all, a.chunks);
     const int waves = A8_WAVES * static_cast<int>(gridDim.y);
     const int lanes = a.d <= 32 ? 8 : a.d <= 64 ? 16 : a.d <= 128 ? 32 : 64;        // of a share's row; the wave takes several shares at a time
     for (int r = threadIdx.x / PL_WAVE + A8_WAVES * blockIdx.y; r < rows; r += waves) {
@@ -807,13 +885,42 @@ static int a8_lds(const void* kernel, size_t lds) {
     return 0;
 }
 
+// Workgroups of the kernel of few rows that a compute unit's registers hold.
+static int a8_held(const void* kernel) {
+    int held = 0;
+    return hipOccupancyMaxActiveBlocksPerMultiprocessor(&held, kernel, A8_WAVES * PL_WAVE, 0) == hipSuccess && held > 0 ? held : 1;
+}
+
 template <int PIECES, int DQ, int RB>
-static int launch_few(const A8Args& a, int rows, hipStream_t stream) {
-    PL_REQUIRE(a8_grid(a, a.S) < (1l << 31), "8-bit attention: %d requests in %d shares are too many for a launch", a.S, a.chunks);
-    const size_t lds = static_cast<size_t>(A8_WAVES) * A8_KEYS * (64 * DQ + 16) * 2 + A8_WAVES * 2 * 16 * RB * 4 + static_cast<size_t>(a.chunk) * 6;
-    if (int e = a8_lds(reinterpret_cast<const void*>(&attention_8bit_few_kernel<PIECES, DQ, RB>), lds)) return e;
+static int launch_few(A8Args a, int rows, hipStream_t stream) {
+    PL_REQUIRE(a8_grid(a, a.S, a.chunks) < (1l << 31), "8-bit attention: %d requests in %d shares are too many for a launch", a.S, a.chunks);
+    auto room = [](int keys) { return static_cast<size_t>(A8_WAVES) * A8_KEYS * (64 * DQ + 16) * 2 + A8_WAVES * 2 * 16 * RB * 4 + static_cast<size_t>(keys) * 6; };
+    a.most = a.chunk;
+    const long longest = static_cast<long>(a.chunk) * a.chunks;
+    if (a.S <= PL_WAVE && a.chunks > 1) {
+        // (as many workgroups a unit as its registers hold, and fewer only where LDS could not hold longer shares of so many)
+        static const int by_registers = a8_held(reinterpret_cast<const void*>(&attention_8bit_few_kernel<PIECES, DQ, RB, true>));
+        int held = by_registers;
+        // (LDS is given out in pieces of 1,280 bytes: three of 54,080, which are less than 160 KB, do not fit)
+        auto fits = [&](int held) { return (160l * 1024 / held / 2560 * 2560 - static_cast<long>(room(0))) / 6 / A8_KEYS * A8_KEYS; };
+        while (held > 1 && fits(held) <= a.chunk) --held;
+        a.places = 256 * held;
+        if (static_cast<long>(a.S) * a.nkv * a.chunks > a.places) a.most = static_cast<int>(max(static_cast<long>(a.chunk), min(longest, min(fits(held), static_cast<long>(A8_MOST_BALANCED)))));
+    }
+    long grid = a8_grid(a, a.S, a.chunks);
+    if (a.most > a.chunk) {
+        // (no more workgroups than the rounds that the longest contexts could take: thousands without work would take turns on the chip)
+        const long rounds = (a.S * ((longest + a.most - 1) / a.most) * a.nkv + a.places - 1) / a.places, shares = min(static_cast<long>(a.S) * a.chunks, rounds * a.places / a.nkv);
+        grid = a8_grid(a, shares, 1);
+    }
+    const size_t lds = room(a.most);
     const unsigned blocks = static_cast<unsigned>(a.S) * a.nkv;
-    attention_8bit_few_kernel<PIECES, DQ, RB><<<static_cast<unsigned>(a8_grid(a, a.S)), A8_WAVES * PL_WAVE, lds, stream>>>(a);
+    auto launch = [&](auto kernel) {
+        if (int e = a8_lds(reinterpret_cast<const void*>(kernel), lds)) return e;
+        kernel<<<static_cast<unsigned>(grid), A8_WAVES * PL_WAVE, lds, stream>>>(a);
+        return 0;
+    };
+    if (int e = a.most > a.chunk ? launch(&attention_8bit_few_kernel<PIECES, DQ, RB, true>) : launch(&attention_8bit_few_kernel<PIECES, DQ, RB, false>)) return e;
     PL_CHECK_LAUNCH("attention_8bit_few");
     if (a.chunks > 1) {
         attention_8bit_merge_kernel<typename A8Type<PIECES>::type><<<dim3(blocks, pl_ceil_div(rows, A8_WAVES)), A8_WAVES * PL_WAVE, 0, stream>>>(a, 16 * RB, 0);
@@ -849,8 +956,8 @@ template <int PIECES, int DT, int NW>
 static int launch_many(const A8Args& a, int few, long blocks, hipStream_t stream) {
     const size_t lds = A8Many<PIECES, DT>::LDS;
     if (int e = a8_lds(reinterpret_cast<const void*>(&attention_8bit_many_kernel<PIECES, DT, NW>), lds)) return e;
-    PL_REQUIRE(a8_grid(a, blocks) < (1l << 31), "8-bit attention: %ld blocks of rows in %d shares are too many for a launch", blocks, a.chunks);
-    attention_8bit_many_kernel<PIECES, DT, NW><<<static_cast<unsigned>(a8_grid(a, blocks)), NW * PL_WAVE, lds, stream>>>(a, few, static_cast<int>(blocks));
+    PL_REQUIRE(a8_grid(a, blocks, a.chunks) < (1l << 31), "8-bit attention: %ld blocks of rows in %d shares are too many for a launch", blocks, a.chunks);
+    attention_8bit_many_kernel<PIECES, DT, NW><<<static_cast<unsigned>(a8_grid(a, blocks, a.chunks)), NW * PL_WAVE, lds, stream>>>(a, few, static_cast<int>(blocks));
     PL_CHECK_LAUNCH("attention_8bit_many");
     if (a.chunks > 1) {
         attention_8bit_merge_kernel<typename A8Type<PIECES>::type><<<dim3(static_cast<unsigned>(blocks * a.nkv), 4 * NW), A8_WAVES * PL_WAVE, 0, stream>>>(a, few, 32 * NW);
@@ -916,7 +1023,7 @@ extern "C" int pl_paged_attention_8bit(const void* q, int q_stride, void* out, c
     const uint32_t magic = static_cast<uint32_t>(((uint64_t{1} << shift) + block - 1) / block);
     A8Args a{q, q_stride, out, static_cast<const int*>(q_start), static_cast<const int*>(q_len), static_cast<const int*>(ctx_len), S, static_cast<const int*>(table), width, block, magic, shift, pool_rows / block,
              static_cast<const uint8_t*>(k_pool), static_cast<const uint8_t*>(v_pool), static_cast<const uint8_t*>(k_scale), static_cast<const uint8_t*>(v_scale),
-             nq, nkv, d, a8_beside(nkv, d), scale * 1.4426950408889634f, window, n, few_chunk, few_chunks, static_cast<float*>(part_acc), static_cast<float*>(part_ml)};
+             nq, nkv, d, a8_beside(nkv, d), scale * 1.4426950408889634f, window, n, few_chunk, few_chunks, few_chunk, 0, static_cast<float*>(part_acc), static_cast<float*>(part_ml)};
     const long group = nq / nkv, longest = max_q_len * group;
     // In a step of portions only what 16 rows hold goes to the kernel of few: those are the single tokens beside them, for which its smallest form is the fastest
     // (15 single tokens at up to 4,600 keys beside a portion: 32 us with it, 91 with the form for 64 rows).

@@ -3050,6 +3050,8 @@ def shares_8bit(n: int, requests: int, max_ctx: int, nq: int, nkv: int, window: 
 
     Few rows: the longest shares, up to 2,048 keys, that still give the chip some 200 workgroups: every share costs a start of some 5 us and leaves a row of results to be put together (8 tokens at 4,000 keys: 20 us in
     shares of 1,024, 25 in 256 or 2,048).  Contexts of up to 640 keys stay whole, which saves the launch that puts shares together (8 tokens at 300 keys: 7.9 us instead of 9.5, at 640 9.8 and 10.8, at 800 11.6 and 10.2).
+    More shares of up to 64 requests than the chip holds are only the shortest: the kernel, which knows every context, makes them as long as fills its rounds (a8_balance), and shorter ones serve steps whose contexts are unlike
+    (one of 16,000 keys and 63 of 300: 27 us from 1,024 on, 32 from 2,048).
     Many rows: as many shares as still leave every workgroup a compute unit of its own, none of fewer than 256 keys.  A share writes and reads its rows' outputs in 32 bits, and two workgroups
     on a unit are no faster than one after the other: 2,048 fresh tokens of 32 heads take 65 us in their 256 blocks and 87 with the keys cut in two, 512 tokens behind 15,500 (64 blocks) 384 us whole, 144 in four, 156 in eight."""
     def of(chunk, reach):
@@ -3061,6 +3063,8 @@ def shares_8bit(n: int, requests: int, max_ctx: int, nq: int, nkv: int, window: 
     chunk = 2048
     while max_ctx > 640 and chunk > 128 and requests * nkv * ((reach + chunk - 1) // chunk) < 200:
         chunk //= 2
+    if requests <= 64 and requests * nkv * ((reach + chunk - 1) // chunk) > 512:
+        chunk = min(chunk, 1024)
     few = of(min(chunk, (max_ctx + 31) // 32 * 32), reach)
     reach = min(max_ctx, abs(window) + 256) if window else max_ctx
     shares = max(1, min(256 // ((n * (nq // nkv) + 255) // 256 * nkv), reach // 256))

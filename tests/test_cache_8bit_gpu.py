@@ -411,6 +411,37 @@ def test_attention_leaves_padding_rows_and_says_a_context_that_is_too_long():
     scene.check(far)
 
 
+UNLIKE = [(1, 1), (1, 5000), (2, 2), (1, 1100), (3, 2300), (0, 40), (1, 4097), (4, 3), (2, 1024), (1, 1025), (3, 700), (1, 3333)]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("nq,nkv,d", [(64, 64, 16), (384, 64, 32), (6, 2, 80)])
+def test_attention_of_more_shares_than_the_chip_holds(dtype, nq, nkv, d):
+    """Contexts so unlike, or said to be so long, that the kernel of few rows cuts them itself."""
+    scene = Scene(UNLIKE, nq, nkv, d, 16, dtype, extra_rows=2)
+    scene.check(scene.run(min_q_len=0))
+    scene.check(scene.run(min_q_len=0, max_ctx=300000))
+    for window in (2500, -3000):
+        scene.check(scene.run(window, min_q_len=0, max_ctx=300000), window)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("requests", [[(1 + s % 5, 1100 + 37 * s) for s in range(60)], [(1, 2500 + s) for s in range(64)], [(1, 900 + 31 * s) for s in range(65)]])
+def test_attention_of_full_rounds_of_shares(dtype, requests):
+    scene = Scene(requests, 64 if requests[1][0] == 2 else 16, 8, 64, 16, dtype)
+    scene.check(scene.run())
+
+
+def test_contexts_that_are_too_long_among_shares_that_the_kernel_cuts():
+    scene = Scene(UNLIKE, 64, 64, 16, 16, torch.bfloat16)
+    out, long = scene.run(min_q_len=0), scene.run(min_q_len=0, max_ctx=2048)
+    for (q, c), at in zip(scene.requests, scene.starts):
+        if c > 2048:
+            assert bool(long[at:at + q].isnan().all())
+            long[at:at + q] = out[at:at + q]
+    scene.check(long)
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_attention_of_large_and_of_equal_scores(dtype):
     scene = Scene([(1, 900), (40, 300)], 8, 2, 64, 16, dtype, largest=200.0)        # weights of one and of zero
