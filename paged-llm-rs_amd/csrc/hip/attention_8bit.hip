@@ -56,6 +56,7 @@ struct A8Args {
     int n, chunk, chunks;     // rows of the step; keys a workgroup, and how many such shares the longest context has
     int most, places;         // few rows: the most keys a workgroup, and how many workgroups the chip holds at once (a8_balance)
     float *part_acc, *part_ml;
+    int parts;                // shares that a row has room for there
 };
 
 __device__ __forceinline__ uint32_t a8_pack2(float lo, float hi) {
@@ -517,7 +518,7 @@ __global__ __launch_bounds__(A8_WAVES * PL_WAVE, (A8Few<PIECES, DQ>::WAVES(RB)))
             __syncthreads();
         }
         if (wave == 0 && out_row[b] >= 0) {
-            const size_t place = static_cast<size_t>(out_row[b]) * a.chunks + share;
+            const size_t place = static_cast<size_t>(out_row[b]) * a.parts + share;
             if (whole_row) {
                 if (!BALANCED && shares > 1) total = NAN;          // (a context longer than the caller said)
                 const float inv = total != 0.f ? 1.f / total : 0.f;
@@ -794,7 +795,7 @@ __global__ __launch_bounds__(NW * PL_WAVE) __attribute__((amdgpu_waves_per_eu(A8
     l += __shfl_xor(l, 32, PL_WAVE);
     if (!live) return;
 
-    const size_t out_row = static_cast<size_t>(q_start + token) * a.nq + head, place = out_row * a.chunks + share;
+    const size_t out_row = static_cast<size_t>(q_start + token) * a.nq + head, place = out_row * a.parts + share;
     float inv = 1.f;
     if (a.chunks == 1) {
         if (shares > 1) l = NAN;              // (a context longer than the caller said)
@@ -815,35 +816,46 @@ __global__ __launch_bounds__(NW * PL_WAVE) __attribute__((amdgpu_waves_per_eu(A8
 }
 
 // ---- shares put together ---------------------------------------------------------------------------------------------------
-// A wave a row and query head: the shares that its block of rows had, in their order.  `per`: rows of a block (0: a request's rows are one block, of at most `few`).
+// A wave a row and query head: the shares that its block of rows had, in their order.  (A request of few rows is one block.)
+// Rows of either kernel, those of many (`tall` workgroups, `many_groups` for a block of `per` rows and a key head) before those of few (`few_groups` for a request and key head): side by side, since each is
+// a chain of reads (512 tokens behind 4,100 beside 15 single ones: 11 us in one launch, 12 and 5 in two).
+struct A8Merge {
+    A8Args many, few;
+    int tall, per, many_groups, few_groups;
+    int above, few_rows;      // rows of a request that are too few for the kernel of many, and as many as the kernel of few took
+};
+
 template <typename T>
-__global__ __launch_bounds__(A8_WAVES * PL_WAVE) void attention_8bit_merge_kernel(A8Args a, int few, int per) {
+__global__ __launch_bounds__(A8_WAVES * PL_WAVE) void attention_8bit_merge_kernel(A8Merge g) {
     const int lane = threadIdx.x % PL_WAVE;
-    const int group = a.nq / a.nkv;
-    const int kvh = blockIdx.x % a.nkv;
-    int seq = blockIdx.x / a.nkv, rb = 0;
-    if (per > 0) {
+    const bool tall = static_cast<int>(blockIdx.x) < g.tall;
+    const A8Args& a = tall ? g.many : g.few;
+    const int group = a.nq / a.nkv, few = tall ? g.above : g.few_rows, per = tall ? g.per : 0;
+    const int every = tall ? g.many_groups : g.few_groups, block = static_cast<int>(blockIdx.x) - (tall ? 0 : g.tall);
+    const int kvh = block / every % a.nkv;
+    int seq = block / every / a.nkv, rb = 0;
+    if (tall) {
         if (!a8_find(a, seq, group, per, few, seq, rb)) return;
     } else if (!a8_brings(a, seq) || a.q_len[seq] * group > few) {
         return;
     }
     const int q_len = a.q_len[seq], start = a.ctx_len[seq] - q_len;
-    const int first_row = rb * per, rows = min(per > 0 ? per : few, q_len * group - first_row);
+    const int first_row = rb * per, rows = min(tall ? per : few, q_len * group - first_row);
     const int lo = pl_first_visible(start + first_row / group, a.window), hi = start + (first_row + rows - 1) / group + 1;
     int all = a8_shares(lo, hi, a.chunk);
-    if (per == 0 && a.most > a.chunk) {
+    if (!tall && a.most > a.chunk) {
         const A8Cut cut = a8_balance(a, group, few);
         all = a8_late(a, hi - lo) ? a.chunks + 1 : __builtin_amdgcn_readlane(cut.shares, seq);
         if (all == 1) return;             // (written as they are)
     }
     const int shares = min(all, a.chunks);
-    const int waves = A8_WAVES * static_cast<int>(gridDim.y);
+    const int waves = A8_WAVES * every;
     const int lanes = a.d <= 32 ? 8 : a.d <= 64 ? 16 : a.d <= 128 ? 32 : 64;        // of a share's row; the wave takes several shares at a time
-    for (int r = threadIdx.x / PL_WAVE + A8_WAVES * blockIdx.y; r < rows; r += waves) {
+    for (int r = threadIdx.x / PL_WAVE + A8_WAVES * (block % every); r < rows; r += waves) {
         const int row = first_row + r;
         const size_t out_row = static_cast<size_t>(a.q_start[seq] + row / group) * a.nq + kvh * group + row % group;
-        const float* ml = a.part_ml + 2 * out_row * a.chunks;
-        const float* acc = a.part_acc + out_row * a.chunks * a.d;
+        const float* ml = a.part_ml + 2 * out_row * a.parts;
+        const float* acc = a.part_acc + out_row * a.parts * a.d;
         float top = -INFINITY;
         for (int s = lane; s < shares; s += PL_WAVE) top = fmaxf(top, ml[2 * s]);
         top = wave_max(top);
@@ -892,7 +904,7 @@ static int a8_held(const void* kernel) {
 }
 
 template <int PIECES, int DQ, int RB>
-static int launch_few(A8Args a, int rows, hipStream_t stream) {
+static int launch_few(A8Args& a, int rows, A8Merge& merge, hipStream_t stream) {
     PL_REQUIRE(a8_grid(a, a.S, a.chunks) < (1l << 31), "8-bit attention: %d requests in %d shares are too many for a launch", a.S, a.chunks);
     auto room = [](int keys) { return static_cast<size_t>(A8_WAVES) * A8_KEYS * (64 * DQ + 16) * 2 + A8_WAVES * 2 * 16 * RB * 4 + static_cast<size_t>(keys) * 6; };
     a.most = a.chunk;
@@ -914,7 +926,6 @@ static int launch_few(A8Args a, int rows, hipStream_t stream) {
         grid = a8_grid(a, shares, 1);
     }
     const size_t lds = room(a.most);
-    const unsigned blocks = static_cast<unsigned>(a.S) * a.nkv;
     auto launch = [&](auto kernel) {
         if (int e = a8_lds(reinterpret_cast<const void*>(kernel), lds)) return e;
         kernel<<<static_cast<unsigned>(grid), A8_WAVES * PL_WAVE, lds, stream>>>(a);
@@ -922,79 +933,78 @@ static int launch_few(A8Args a, int rows, hipStream_t stream) {
     };
     if (int e = a.most > a.chunk ? launch(&attention_8bit_few_kernel<PIECES, DQ, RB, true>) : launch(&attention_8bit_few_kernel<PIECES, DQ, RB, false>)) return e;
     PL_CHECK_LAUNCH("attention_8bit_few");
-    if (a.chunks > 1) {
-        attention_8bit_merge_kernel<typename A8Type<PIECES>::type><<<dim3(blocks, pl_ceil_div(rows, A8_WAVES)), A8_WAVES * PL_WAVE, 0, stream>>>(a, 16 * RB, 0);
-        PL_CHECK_LAUNCH("attention_8bit_merge");
-    }
+    merge.few_groups = pl_ceil_div(rows, A8_WAVES);
+    merge.few_rows = 16 * RB;
     return 0;
 }
 
 template <int PIECES, int DQ>
-static int launch_few(const A8Args& a, int rows, hipStream_t stream) {
+static int launch_few(A8Args& a, int rows, A8Merge& merge, hipStream_t stream) {
     constexpr int MOST = A8Few<PIECES, DQ>::BLOCKS;
-    if (rows <= 16 || MOST == 1) return launch_few<PIECES, DQ, 1>(a, rows, stream);
+    if (rows <= 16 || MOST == 1) return launch_few<PIECES, DQ, 1>(a, rows, merge, stream);
     if constexpr (MOST >= 2)
-        if (rows <= 32 || MOST == 2) return launch_few<PIECES, DQ, 2>(a, rows, stream);
+        if (rows <= 32 || MOST == 2) return launch_few<PIECES, DQ, 2>(a, rows, merge, stream);
     if constexpr (MOST >= 4) {
-        if (rows <= 48) return launch_few<PIECES, DQ, 3>(a, rows, stream);
-        return launch_few<PIECES, DQ, 4>(a, rows, stream);
+        if (rows <= 48) return launch_few<PIECES, DQ, 3>(a, rows, merge, stream);
+        return launch_few<PIECES, DQ, 4>(a, rows, merge, stream);
     }
     return 0;
 }
 
 template <int PIECES>
-static int launch_few(const A8Args& a, int rows, hipStream_t stream) {
+static int launch_few(A8Args& a, int rows, A8Merge& merge, hipStream_t stream) {
     switch (pl_ceil_div(a.d, 64)) {
-        case 1: return launch_few<PIECES, 1>(a, rows, stream);
-        case 2: return launch_few<PIECES, 2>(a, rows, stream);
-        case 3: return launch_few<PIECES, 3>(a, rows, stream);
-        default: return launch_few<PIECES, 4>(a, rows, stream);
+        case 1: return launch_few<PIECES, 1>(a, rows, merge, stream);
+        case 2: return launch_few<PIECES, 2>(a, rows, merge, stream);
+        case 3: return launch_few<PIECES, 3>(a, rows, merge, stream);
+        default: return launch_few<PIECES, 4>(a, rows, merge, stream);
     }
 }
 
 template <int PIECES, int DT, int NW>
-static int launch_many(const A8Args& a, int few, long blocks, hipStream_t stream) {
+static int launch_many(const A8Args& a, int few, long blocks, A8Merge& merge, hipStream_t stream) {
     const size_t lds = A8Many<PIECES, DT>::LDS;
     if (int e = a8_lds(reinterpret_cast<const void*>(&attention_8bit_many_kernel<PIECES, DT, NW>), lds)) return e;
-    PL_REQUIRE(a8_grid(a, blocks, a.chunks) < (1l << 31), "8-bit attention: %ld blocks of rows in %d shares are too many for a launch", blocks, a.chunks);
+    PL_REQUIRE(a8_grid(a, blocks, a.chunks) < (1l << 31) && blocks * a.nkv * 4 * NW < (1l << 31), "8-bit attention: %ld blocks of rows in %d shares are too many for a launch", blocks, a.chunks);
     attention_8bit_many_kernel<PIECES, DT, NW><<<static_cast<unsigned>(a8_grid(a, blocks, a.chunks)), NW * PL_WAVE, lds, stream>>>(a, few, static_cast<int>(blocks));
     PL_CHECK_LAUNCH("attention_8bit_many");
     if (a.chunks > 1) {
-        attention_8bit_merge_kernel<typename A8Type<PIECES>::type><<<dim3(static_cast<unsigned>(blocks * a.nkv), 4 * NW), A8_WAVES * PL_WAVE, 0, stream>>>(a, few, 32 * NW);
-        PL_CHECK_LAUNCH("attention_8bit_merge");
+        merge.per = 32 * NW;
+        merge.many_groups = 4 * NW;
+        merge.tall = static_cast<int>(blocks * a.nkv * merge.many_groups);
     }
     return 0;
 }
 
 template <int PIECES, int DT, int NW>
-static int launch_many_blocks(const A8Args& a, int few, int max_q_len, hipStream_t stream) {
+static int launch_many_blocks(const A8Args& a, int few, int max_q_len, A8Merge& merge, hipStream_t stream) {
     const int group = a.nq / a.nkv;
     // blocks of rows: one a request for what is left over, and the whole ones
     const long most = static_cast<long>(a.S) * ((static_cast<long>(max_q_len) * group + 32 * NW - 1) / (32 * NW)), all = a.S + static_cast<long>(a.n) * group / (32 * NW);
-    return launch_many<PIECES, DT, NW>(a, few, most < all ? most : all, stream);
+    return launch_many<PIECES, DT, NW>(a, few, most < all ? most : all, merge, stream);
 }
 
 // Four waves a workgroup where eight's registers or LDS leave no second one beside it anyway (32 bits, heads of more than 128) or where two of four fit a unit (heads of up to 64: 2 prompts of 1,500 to 2,000 tokens,
 // 16 heads over 8, 45 us with eight, 40 with four); else eight, which widen a tile for 256 rows, but for so few rows that workgroups of 128 do not fill the chip either (512 tokens of 16 heads over 8: 23.5 and 20.8 us).
 template <int PIECES, int DT>
-static int launch_many(const A8Args& a, int few, int max_q_len, hipStream_t stream) {
+static int launch_many(const A8Args& a, int few, int max_q_len, A8Merge& merge, hipStream_t stream) {
     if constexpr (PIECES == 1 && (DT == 3 || DT == 4)) {
         const long blocks = (static_cast<long>(a.n) * (a.nq / a.nkv) + 127) / 128 * a.nkv * a.chunks;
-        if (blocks > 256) return launch_many_blocks<PIECES, DT, 8>(a, few, max_q_len, stream);
+        if (blocks > 256) return launch_many_blocks<PIECES, DT, 8>(a, few, max_q_len, merge, stream);
     }
-    return launch_many_blocks<PIECES, DT, 4>(a, few, max_q_len, stream);
+    return launch_many_blocks<PIECES, DT, 4>(a, few, max_q_len, merge, stream);
 }
 
 template <int PIECES>
-static int launch_many(const A8Args& a, int few, int max_q_len, hipStream_t stream) {
+static int launch_many(const A8Args& a, int few, int max_q_len, A8Merge& merge, hipStream_t stream) {
     switch (pl_ceil_div(a.d, 32)) {
-        case 1: return launch_many<PIECES, 1>(a, few, max_q_len, stream);
-        case 2: return launch_many<PIECES, 2>(a, few, max_q_len, stream);
-        case 3: return launch_many<PIECES, 3>(a, few, max_q_len, stream);
-        case 4: return launch_many<PIECES, 4>(a, few, max_q_len, stream);
+        case 1: return launch_many<PIECES, 1>(a, few, max_q_len, merge, stream);
+        case 2: return launch_many<PIECES, 2>(a, few, max_q_len, merge, stream);
+        case 3: return launch_many<PIECES, 3>(a, few, max_q_len, merge, stream);
+        case 4: return launch_many<PIECES, 4>(a, few, max_q_len, merge, stream);
         case 5:
-        case 6: return launch_many<PIECES, 6>(a, few, max_q_len, stream);
-        default: return launch_many<PIECES, 8>(a, few, max_q_len, stream);
+        case 6: return launch_many<PIECES, 6>(a, few, max_q_len, merge, stream);
+        default: return launch_many<PIECES, 8>(a, few, max_q_len, merge, stream);
     }
 }
 
@@ -1023,7 +1033,7 @@ extern "C" int pl_paged_attention_8bit(const void* q, int q_stride, void* out, c
     const uint32_t magic = static_cast<uint32_t>(((uint64_t{1} << shift) + block - 1) / block);
     A8Args a{q, q_stride, out, static_cast<const int*>(q_start), static_cast<const int*>(q_len), static_cast<const int*>(ctx_len), S, static_cast<const int*>(table), width, block, magic, shift, pool_rows / block,
              static_cast<const uint8_t*>(k_pool), static_cast<const uint8_t*>(v_pool), static_cast<const uint8_t*>(k_scale), static_cast<const uint8_t*>(v_scale),
-             nq, nkv, d, a8_beside(nkv, d), scale * 1.4426950408889634f, window, n, few_chunk, few_chunks, few_chunk, 0, static_cast<float*>(part_acc), static_cast<float*>(part_ml)};
+             nq, nkv, d, a8_beside(nkv, d), scale * 1.4426950408889634f, window, n, few_chunk, few_chunks, few_chunk, 0, static_cast<float*>(part_acc), static_cast<float*>(part_ml), max(few_chunks, many_chunks)};
     const long group = nq / nkv, longest = max_q_len * group;
     // In a step of portions only what 16 rows hold goes to the kernel of few: those are the single tokens beside them, for which its smallest form is the fastest
     // (15 single tokens at up to 4,600 keys beside a portion: 32 us with it, 91 with the form for 64 rows).
@@ -1031,15 +1041,22 @@ extern "C" int pl_paged_attention_8bit(const void* q, int q_stride, void* out, c
     if (longest > few) few = 16;
     const hipStream_t on = static_cast<hipStream_t>(stream);
     const bool f32 = dtype == PL_DTYPE_F32;
+    A8Merge merge{a, a, 0, 0, 1, 1, few, 0};
     if (longest > few) {
-        a.chunk = many_chunk;
-        a.chunks = many_chunks;
-        if (int e = f32 ? launch_many<3>(a, few, max_q_len, on) : launch_many<1>(a, few, max_q_len, on)) return e;
+        merge.many.chunk = many_chunk;
+        merge.many.chunks = many_chunks;
+        if (int e = f32 ? launch_many<3>(merge.many, few, max_q_len, merge, on) : launch_many<1>(merge.many, few, max_q_len, merge, on)) return e;
     }
+    long groups = merge.tall;
     if (min_q_len * group <= few) {
-        a.chunk = few_chunk;
-        a.chunks = few_chunks;
-        return f32 ? launch_few<3>(a, static_cast<int>(min(longest, static_cast<long>(few))), on) : launch_few<1>(a, static_cast<int>(min(longest, static_cast<long>(few))), on);
+        const int rows = static_cast<int>(min(longest, static_cast<long>(few)));
+        if (int e = f32 ? launch_few<3>(merge.few, rows, merge, on) : launch_few<1>(merge.few, rows, merge, on)) return e;
+        if (few_chunks > 1) groups += static_cast<long>(S) * nkv * merge.few_groups;
     }
+    if (groups == 0) return 0;
+    PL_REQUIRE(groups < (1l << 31), "8-bit attention: shares of %d requests are too many for a launch", S);
+    if (f32) attention_8bit_merge_kernel<float><<<static_cast<unsigned>(groups), A8_WAVES * PL_WAVE, 0, on>>>(merge);
+    else attention_8bit_merge_kernel<bf16_t><<<static_cast<unsigned>(groups), A8_WAVES * PL_WAVE, 0, on>>>(merge);
+    PL_CHECK_LAUNCH("attention_8bit_merge");
     return 0;
 }
