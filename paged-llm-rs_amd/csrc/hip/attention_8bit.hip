@@ -57,6 +57,7 @@ struct A8Args {
     int most, places;         // few rows: the most keys a workgroup, and how many workgroups the chip holds at once (a8_balance)
     float *part_acc, *part_ml;
     int parts;                // shares that a row has room for there
+    int* cut;                 // behind them: the shares of each request as a8_balance cut them, more than `chunks` for a context longer than the caller said
 };
 
 __device__ __forceinline__ uint32_t a8_pack2(float lo, float hi) {
@@ -290,7 +291,9 @@ __global__ __launch_bounds__(A8_WAVES * PL_WAVE, (A8Few<PIECES, DQ>::WAVES(RB)))
         share = number - (__builtin_amdgcn_readlane(end, seq) - shares);
         hi = start + q_len;
         k_base = lo + share * size;
+        const bool first = share == 0 && kvh == 0 && tid == 0;
         if (a8_late(a, hi - lo)) shares = a.chunks + 1;
+        if (first) a.cut[seq] = shares;
     } else {
         if (!a8_brings(a, seq) || a.q_len[seq] * group > 16 * RB) return;
         q_len = a.q_len[seq];
@@ -844,8 +847,7 @@ __global__ __launch_bounds__(A8_WAVES * PL_WAVE) void attention_8bit_merge_kerne
     const int lo = pl_first_visible(start + first_row / group, a.window), hi = start + (first_row + rows - 1) / group + 1;
     int all = a8_shares(lo, hi, a.chunk);
     if (!tall && a.most > a.chunk) {
-        const A8Cut cut = a8_balance(a, group, few);
-        all = a8_late(a, hi - lo) ? a.chunks + 1 : __builtin_amdgcn_readlane(cut.shares, seq);
+        all = a.cut[seq];
         if (all == 1) return;             // (written as they are)
     }
     const int shares = min(all, a.chunks);
@@ -856,24 +858,29 @@ __global__ __launch_bounds__(A8_WAVES * PL_WAVE) void attention_8bit_merge_kerne
         const size_t out_row = static_cast<size_t>(a.q_start[seq] + row / group) * a.nq + kvh * group + row % group;
         const float* ml = a.part_ml + 2 * out_row * a.parts;
         const float* acc = a.part_acc + out_row * a.parts * a.d;
-        float top = -INFINITY;
-        for (int s = lane; s < shares; s += PL_WAVE) top = fmaxf(top, ml[2 * s]);
-        top = wave_max(top);
-        const float base2 = top == -INFINITY ? 0.f : top;
-        float total = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
-        const int at = 4 * (lane % lanes);
-#pragma unroll 4
-        for (int s = lane / lanes; s < shares; s += PL_WAVE / lanes) {
-            const float w = __builtin_amdgcn_exp2f(ml[2 * s] - base2);
-            total += w * ml[2 * s + 1];
-            if (at < a.d) {
-                const a8_f32x4 y = *reinterpret_cast<const a8_f32x4*>(acc + static_cast<size_t>(s) * a.d + at);
+        float top = -INFINITY, total = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
+        const int at = 4 * (lane % lanes), from_at = min(at, a.d - 4);
+        for (int base = 0; base < shares; base += PL_WAVE) {
+            // (a lane has one share's maximum and sum; the shares' rows are asked for without regard to them, eight reads at once)
+            const int here = min(shares - base, PL_WAVE), own = min(lane, here - 1);
+            const float m = lane < here ? ml[2 * (base + own)] : -INFINITY, l = ml[2 * (base + own) + 1];
+            const float grown = fmaxf(top, wave_max(m)), from = grown == -INFINITY ? 0.f : grown;
+            const float weight = __builtin_amdgcn_exp2f(m - from), alpha = __builtin_amdgcn_exp2f(top - from);
+            top = grown;
+            total = total * alpha + (lane < here ? weight * l : 0.f);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) x[e] += w * y[e];
+            for (int e = 0; e < 4; ++e) x[e] *= alpha;
+#pragma unroll 8
+            for (int i = 0; i < here; i += PL_WAVE / lanes) {
+                const int s = i + lane / lanes;
+                const a8_f32x4 y = *reinterpret_cast<const a8_f32x4*>(acc + static_cast<size_t>(base + min(s, here - 1)) * a.d + from_at);
+                const float w = __shfl(weight, s % PL_WAVE, PL_WAVE);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[e] += s < here ? w * y[e] : 0.f;
             }
         }
+        total = wave_sum(total);
         for (int off = lanes; off < PL_WAVE; off <<= 1) {
-            total += __shfl_xor(total, off, PL_WAVE);
 #pragma unroll
             for (int e = 0; e < 4; ++e) x[e] += __shfl_xor(x[e], off, PL_WAVE);
         }
@@ -1015,7 +1022,8 @@ extern "C" int pl_paged_attention_8bit_few(int d, int dtype) {
     return 16 * (dq <= 2 ? A8Few<1, 2>::BLOCKS : A8Few<1, 3>::BLOCKS);
 }
 
-// `few_rows`, `many_rows`: the most rows of a request that goes to the kernel of few rows, or 0, and the most of one that goes to the kernel of many, or 0; each has shares of its own size.
+// The kernel of few rows and that of many have shares of their own size.  Where either has more than one: `part_acc` has room for d floats for each of them (the larger number) and each of the n * nq rows,
+// `part_ml` for two, and for S more behind those.
 extern "C" int pl_paged_attention_8bit(const void* q, int q_stride, void* out, const void* q_start, const void* q_len, const void* ctx_len, int S, int n, int max_q_len, int min_q_len,
                                        const void* table, int width, int block, int pool_rows, const void* k_pool, const void* v_pool, const void* k_scale,
                                        const void* v_scale, int nq, int nkv, int d, float scale, int window, int few_chunk, int few_chunks, int many_chunk, int many_chunks,
@@ -1033,7 +1041,8 @@ extern "C" int pl_paged_attention_8bit(const void* q, int q_stride, void* out, c
     const uint32_t magic = static_cast<uint32_t>(((uint64_t{1} << shift) + block - 1) / block);
     A8Args a{q, q_stride, out, static_cast<const int*>(q_start), static_cast<const int*>(q_len), static_cast<const int*>(ctx_len), S, static_cast<const int*>(table), width, block, magic, shift, pool_rows / block,
              static_cast<const uint8_t*>(k_pool), static_cast<const uint8_t*>(v_pool), static_cast<const uint8_t*>(k_scale), static_cast<const uint8_t*>(v_scale),
-             nq, nkv, d, a8_beside(nkv, d), scale * 1.4426950408889634f, window, n, few_chunk, few_chunks, few_chunk, 0, static_cast<float*>(part_acc), static_cast<float*>(part_ml), max(few_chunks, many_chunks)};
+             nq, nkv, d, a8_beside(nkv, d), scale * 1.4426950408889634f, window, n, few_chunk, few_chunks, few_chunk, 0, static_cast<float*>(part_acc), static_cast<float*>(part_ml), max(few_chunks, many_chunks), nullptr};
+    if (part_ml) a.cut = reinterpret_cast<int*>(a.part_ml + 2l * n * nq * a.parts);
     const long group = nq / nkv, longest = max_q_len * group;
     // In a step of portions only what 16 rows hold goes to the kernel of few: those are the single tokens beside them, for which its smallest form is the fastest
     // (15 single tokens at up to 4,600 keys beside a portion: 32 us with it, 91 with the form for 64 rows).
@@ -1042,16 +1051,17 @@ extern "C" int pl_paged_attention_8bit(const void* q, int q_stride, void* out, c
     const hipStream_t on = static_cast<hipStream_t>(stream);
     const bool f32 = dtype == PL_DTYPE_F32;
     A8Merge merge{a, a, 0, 0, 1, 1, few, 0};
+    long groups = 0;
+    if (min_q_len * group <= few) {
+        const int rows = static_cast<int>(min(longest, static_cast<long>(few)));
+        if (int e = f32 ? launch_few<3>(merge.few, rows, merge, on) : launch_few<1>(merge.few, rows, merge, on)) return e;
+        if (few_chunks > 1) groups = static_cast<long>(S) * nkv * merge.few_groups;
+    }
     if (longest > few) {
         merge.many.chunk = many_chunk;
         merge.many.chunks = many_chunks;
         if (int e = f32 ? launch_many<3>(merge.many, few, max_q_len, merge, on) : launch_many<1>(merge.many, few, max_q_len, merge, on)) return e;
-    }
-    long groups = merge.tall;
-    if (min_q_len * group <= few) {
-        const int rows = static_cast<int>(min(longest, static_cast<long>(few)));
-        if (int e = f32 ? launch_few<3>(merge.few, rows, merge, on) : launch_few<1>(merge.few, rows, merge, on)) return e;
-        if (few_chunks > 1) groups += static_cast<long>(S) * nkv * merge.few_groups;
+        groups += merge.tall;
     }
     if (groups == 0) return 0;
     PL_REQUIRE(groups < (1l << 31), "8-bit attention: shares of %d requests are too many for a launch", S);

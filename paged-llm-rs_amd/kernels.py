@@ -3105,7 +3105,7 @@ def paged_attention_8bit(q: torch.Tensor, q_row_stride: int, out: torch.Tensor, 
     chunks = max(few_shares, many_shares)
     acc = ml = 0
     if chunks > 1:
-        room = torch.empty(n * nq * chunks * (d + 2), dtype=torch.float32, device=q.device)
+        room = torch.empty(n * nq * chunks * (d + 2) + S, dtype=torch.float32, device=q.device)
         acc = room.data_ptr()
         ml = acc + 4 * n * nq * chunks * d
     _check(library().pl_paged_attention_8bit(
