@@ -923,7 +923,7 @@ static int launch_few(A8Args& a, int rows, A8Merge& merge, hipStream_t stream) {
         // (LDS is given out in pieces of 1,280 bytes: three of 54,080, which are less than 160 KB, do not fit)
         auto fits = [&](int held) { return (160l * 1024 / held / 2560 * 2560 - static_cast<long>(room(0))) / 6 / A8_KEYS * A8_KEYS; };
         while (held > 1 && fits(held) <= a.chunk) --held;
-        a.places = 256 * held;
+        a.places = pl_compute_units() * held;
         if (static_cast<long>(a.S) * a.nkv * a.chunks > a.places) a.most = static_cast<int>(max(static_cast<long>(a.chunk), min(longest, min(fits(held), static_cast<long>(A8_MOST_BALANCED)))));
     }
     long grid = a8_grid(a, a.S, a.chunks);

@@ -3045,15 +3045,16 @@ def qk_norm_rope_kv_write_8bit(qkv: torch.Tensor, q: torch.Tensor | None, q_gain
 
 
 @functools.lru_cache(maxsize=4096)
-def shares_8bit(n: int, requests: int, max_ctx: int, nq: int, nkv: int, window: int = 0) -> tuple:
+def shares_8bit(n: int, requests: int, max_ctx: int, nq: int, nkv: int, window: int = 0, d: int = 128, f32: bool = False) -> tuple:
     """(keys a share, shares) of the 8-bit attention's kernel of few rows, and the same of its kernel of many.
 
     Few rows: the longest shares, up to 2,048 keys, that still give the chip some 200 workgroups: every share costs a start of some 5 us and leaves a row of results to be put together (8 tokens at 4,000 keys: 20 us in
     shares of 1,024, 25 in 256 or 2,048).  Contexts of up to 640 keys stay whole, which saves the launch that puts shares together (8 tokens at 300 keys: 7.9 us instead of 9.5, at 640 9.8 and 10.8, at 800 11.6 and 10.2).
     More shares of up to 64 requests than the chip holds are only the shortest: the kernel, which knows every context, makes them as long as fills its rounds (a8_balance), and shorter ones serve steps whose contexts are unlike
     (one of 16,000 keys and 63 of 300: 27 us from 1,024 on, 32 from 2,048).
-    Many rows: as many shares as still leave every workgroup a compute unit of its own, none of fewer than 256 keys.  A share writes and reads its rows' outputs in 32 bits, and two workgroups
-    on a unit are no faster than one after the other: 2,048 fresh tokens of 32 heads take 65 us in their 256 blocks and 87 with the keys cut in two, 512 tokens behind 15,500 (64 blocks) 384 us whole, 144 in four, 156 in eight."""
+    Many rows: the number with the least estimate among those that leave every workgroup a compute unit of its own (two on a unit are no faster than one after the other: 2,048 fresh tokens of 32 heads take 65 us in
+    their 256 blocks and 87 with the keys cut in two), none of fewer than 128 keys.  64 keys take a workgroup 1.5 us at heads of 128, twice that in 32 bits; shares cost a launch and what is written and read of every row in 32 bits
+    (16 heads over 8: 2 prompts of 610 to 687 24 us whole, 39 in two; 512 tokens behind 15,500 384 us whole, 144 in four, 156 in eight; heads of 256 in 32 bits, 5 prompts of 778, 127 and 167)."""
     def of(chunk, reach):
         # shares begin at whole ones of them, so what a block of rows sees under a mask may touch one more than it fills
         every = (max_ctx + chunk - 1) // chunk
@@ -3067,7 +3068,11 @@ def shares_8bit(n: int, requests: int, max_ctx: int, nq: int, nkv: int, window: 
         chunk = min(chunk, 1024)
     few = of(min(chunk, (max_ctx + 31) // 32 * 32), reach)
     reach = min(max_ctx, abs(window) + 256) if window else max_ctx
-    shares = max(1, min(256 // ((n * (nq // nkv) + 255) // 256 * nkv), reach // 256))
+    # (what a compute unit holds: 256 rows, or 128 where their outputs take all registers; most requests beside a portion bring one token)
+    rows = 128 if d > (96 if f32 else 128) else 256
+    most = max(1, min(256 // ((max(n - requests + 1, 1) * (nq // nkv) + rows - 1) // rows * nkv), reach // 128))
+    stretch = 1.5 * (2 if f32 else 1) * (d if d <= 128 else 1.5 * d) / 128          # (microseconds for 64 keys)
+    shares = min(range(1, most + 1), key=lambda count: reach / 64 / count * stretch + (9 + n * nq * count * d * 8 / 3.5e6 if count > 1 else 0))
     return few + of((reach + 64 * shares - 1) // (64 * shares) * 64 if shares > 1 else (max_ctx + 63) // 64 * 64, reach)
 
 
@@ -3101,7 +3106,7 @@ def paged_attention_8bit(q: torch.Tensor, q_row_stride: int, out: torch.Tensor, 
     queries, results = _fits(q, "query buffer", q.dtype, n * q_row_stride, device), _fits(out, "attention output", q.dtype, n * nq * d, device, (n, nq * d))
     if q_row_stride % 8 or (queries | results) % 16:
         raise TensorError("query rows and outputs for an 8-bit cache begin at whole 16 bytes")
-    few, few_shares, many, many_shares = shares_8bit(n, S, max_ctx, nq, nkv, window)
+    few, few_shares, many, many_shares = shares_8bit(n, S, max_ctx, nq, nkv, window, d, code == F32)
     chunks = max(few_shares, many_shares)
     acc = ml = 0
     if chunks > 1:
