@@ -255,8 +255,8 @@ __device__ __forceinline__ float a8_max_quarters(float v) {
 // A workgroup takes the RB blocks of 16 rows of one request and key head and one share of the keys; its waves take tiles of 32 keys in turn, each with a running maximum and sum, and meet at the end.
 // Keys go from memory into the registers that the product reads (a lane reads 16 bytes of one key: the contraction may go through a head's values in any order, so the
 // queries are laid out to match); values go through a piece of LDS that belongs to the wave, so the loop has no barrier.  The next tile's bytes are on their way while a tile is worked on.
-// Bound by memory: 64 single tokens of 32 heads over 8 at contexts of 1,000 to 12,000 read 857 MB in 203 us, 4.2 TB/s (a copy of 4 GB moves 4.6, pieces of 128 bytes as these are read at 5.3), and their shares are
-// put together in another 7.  A wave has one key head: four heads' pieces side by side would be read at 6.2 TB/s, but with four times the shares to put together.
+// Bound by memory: 64 single tokens of 32 heads over 8 at contexts of 1,000 to 12,000 read 857 MB in 190 us, 4.5 TB/s (a copy of 4 GB moves 4.6, pieces of 128 bytes as these are read at 5.3), and their shares are
+// put together in another 6.  A wave has one key head: four heads' pieces side by side would be read at 6.2 TB/s, but with four times the shares to put together.
 //   S^T = K . Q^T: v_mfma_f32_16x16x32_bf16, twice for 32 keys; a lane has for row lane % 16 the keys 4 (lane / 16) .. + 3 of both.  DQ: the head is padded to 64 DQ values.
 //   BALANCED: with the shares of a8_balance.  (A build of its own: the one for shares as the caller cut them loses 0.4 to 1 us of 12 to 20 to what is only compiled in.)
 template <int PIECES, int DQ, int RB, bool BALANCED>
