@@ -3051,7 +3051,7 @@ def shares_8bit(n: int, requests: int, max_ctx: int, nq: int, nkv: int, window: 
     Few rows: the longest shares, up to 2,048 keys, that still give the chip some 200 workgroups: every share costs a start of some 5 us and leaves a row of results to be put together (8 tokens at 4,000 keys: 20 us in
     shares of 1,024, 25 in 256 or 2,048).  Contexts of up to 640 keys stay whole, which saves the launch that puts shares together (8 tokens at 300 keys: 7.9 us instead of 9.5, at 640 9.8 and 10.8, at 800 11.6 and 10.2).
     More shares of up to 64 requests than the chip holds are only the shortest: the kernel, which knows every context, makes them as long as fills its rounds (a8_balance), and shorter ones serve steps whose contexts are unlike
-    (one of 16,000 keys and 63 of 300: 27 us from 1,024 on, 32 from 2,048).
+    (one of 16,000 keys and 63 of 300: 27 us from 1,024 on, 32 from 2,048), as long as what they leave for the last launch stays within 256 MB.
     Many rows: the number with the least estimate among those that leave every workgroup a compute unit of its own (two on a unit are no faster than one after the other: 2,048 fresh tokens of 32 heads take 65 us in
     their 256 blocks and 87 with the keys cut in two), none of fewer than 128 keys.  64 keys take a workgroup 1.5 us at heads of 128, twice that in 32 bits; shares cost a launch and what is written and read of every row in 32 bits
     (16 heads over 8: 2 prompts of 610 to 687 24 us whole, 39 in two; 512 tokens behind 15,500 384 us whole, 144 in four, 156 in eight; heads of 256 in 32 bits, 5 prompts of 778, 127 and 167)."""
@@ -3064,7 +3064,7 @@ def shares_8bit(n: int, requests: int, max_ctx: int, nq: int, nkv: int, window: 
     chunk = 2048
     while max_ctx > 640 and chunk > 128 and requests * nkv * ((reach + chunk - 1) // chunk) < 200:
         chunk //= 2
-    if requests <= 64 and requests * nkv * ((reach + chunk - 1) // chunk) > 512:
+    if requests <= 64 and requests * nkv * ((reach + chunk - 1) // chunk) > 512 and n * nq * (reach // 1024 + 2) * d <= 2 ** 26:
         chunk = min(chunk, 1024)
     few = of(min(chunk, (max_ctx + 31) // 32 * 32), reach)
     reach = min(max_ctx, abs(window) + 256) if window else max_ctx
