@@ -3051,6 +3051,7 @@ def shares_8bit(n: int, requests: int, max_ctx: int, nq: int, nkv: int, window: 
     Few rows: the longest shares, up to 2,048 keys, that still give the chip some 200 workgroups: every share costs a start of some 5 us and leaves a row of results to be put together (8 tokens at 4,000 keys: 20 us in
     shares of 1,024, 25 in 256 or 2,048).  Contexts of up to 640 keys stay whole, which saves the launch that puts shares together (8 tokens at 300 keys: 7.9 us instead of 9.5, at 640 9.8 and 10.8, at 800 11.6 and 10.2).
     128 keys take a workgroup some 0.9 us, a share 0.1 where they are put together: none is cut where that costs more than it saves (one token of 12 heads of 96 at 4,000 keys: 12.8 us in 16 shares, 15.5 in 32).
+    And where they can, shares are as many as compute units: 8 tokens of 32 heads over 8 at 3,000 keys 20.3 us in 256, 23.5 in 384, 22.1 in 192.
     More shares of up to 64 requests than the chip holds are only the shortest: the kernel, which knows every context, makes them as long as fills its rounds (a8_balance), and shorter ones serve steps whose contexts are unlike
     (one of 16,000 keys and 63 of 300: 27 us from 1,024 on, 32 from 2,048), as long as what they leave for the last launch stays within 256 MB.
     Many rows: the number with the least estimate among those that leave every workgroup a compute unit of its own (two on a unit are no faster than one after the other: 2,048 fresh tokens of 32 heads take 65 us in
@@ -3065,6 +3066,10 @@ def shares_8bit(n: int, requests: int, max_ctx: int, nq: int, nkv: int, window: 
     chunk = 2048
     while max_ctx > 640 and chunk > 128 and requests * nkv * ((reach + chunk - 1) // chunk) < 200 and chunk * chunk > 28 * reach:
         chunk //= 2
+    units = 256 // (requests * nkv)
+    if max_ctx > 640 and units > 0 and not window:
+        even = (reach + 32 * units - 1) // (32 * units) * 32
+        chunk = even if chunk <= even < min(2 * chunk, 2048) else chunk
     if requests <= 64 and requests * nkv * ((reach + chunk - 1) // chunk) > 512 and n * nq * (reach // 1024 + 2) * d <= 2 ** 26:
         chunk = min(chunk, 1024)
     few = of(min(chunk, (max_ctx + 31) // 32 * 32), reach)
