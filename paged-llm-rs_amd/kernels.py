@@ -3077,8 +3077,10 @@ def shares_8bit(n: int, requests: int, max_ctx: int, nq: int, nkv: int, window: 
     # (what a compute unit holds: 256 rows, or 128 where their outputs take all registers; most requests beside a portion bring one token)
     rows = 128 if d > (96 if f32 else 128) else 256
     most = max(1, min(256 // ((max(n - requests + 1, 1) * (nq // nkv) + rows - 1) // rows * nkv), reach // 128))
-    stretch = 1.5 * (2 if f32 else 1) * (d if d <= 128 else 1.5 * d) / 128          # (microseconds for 64 keys)
-    shares = min(range(1, most + 1), key=lambda count: reach / 64 / count * stretch + (9 + n * nq * count * d * 8 / 3.5e6 if count > 1 else 0))
+    whole = reach / 64 * 1.5 * (2 if f32 else 1) * (d if d <= 128 else 1.5 * d) / 128          # (microseconds)
+    each = n * nq * d * 8 / 3.5e6
+    least = int(math.sqrt(whole / each))            # whole / shares + each * shares is least here or at the next number
+    shares = min({1, min(max(least, 1), most), min(least + 1, most)}, key=lambda count: whole / count + (9 + each * count if count > 1 else 0))
     return few + of((reach + 64 * shares - 1) // (64 * shares) * 64 if shares > 1 else (max_ctx + 63) // 64 * 64, reach)
 
 
