@@ -63,3 +63,17 @@ def test_the_shares_cover_every_context():
                             # a stretch of `reach` keys anywhere in the context touches at most so many shares
                             touched = min(-(-max_ctx // chunk), (reach - 1) // chunk + 2 if window else -(-max_ctx // chunk))
                             assert shares >= touched
+
+
+@pytest.mark.parametrize("f32", [False, True])
+@pytest.mark.parametrize("d", [16, 96, 128, 256])
+def test_the_shares_of_other_heads_cover_every_context(d, f32):
+    for n, requests in ((1, 1), (64, 64), (527, 16), (4000, 5), (70000, 600)):
+        for max_ctx in (1, 640, 641, 1500, 3100, 24000, 1 << 20):
+            for nq, nkv in ((16, 8), (64, 8), (8, 1), (300, 100)):
+                for window in (0, 100, -3000):
+                    few, few_shares, many, many_shares = kernels.shares_8bit(n, requests, max_ctx, nq, nkv, window, d, f32)
+                    assert few % 32 == 0 and 32 <= few <= 2048 and many % 64 == 0 and many >= 64
+                    for chunk, shares, tokens in ((few, few_shares, 64), (many, many_shares, 256)):
+                        reach = max_ctx if window == 0 else min(max_ctx, abs(window) + tokens)
+                        assert shares >= min(-(-max_ctx // chunk), (reach - 1) // chunk + 2 if window else -(-max_ctx // chunk))
