@@ -57,6 +57,7 @@ struct A8Args {
     int most, places;         // few rows: the most keys a workgroup, and how many workgroups the chip holds at once (a8_balance)
     float *part_acc, *part_ml;
     int parts;                // shares that a row has room for there
+    int rows_each;            // few rows: the room is numbered by request and key head with so many rows for each, or (0) by the step's rows and heads
     int* cut;                 // behind them: the shares of each request as a8_balance cut them, more than `chunks` for a context longer than the caller said
 };
 
@@ -104,6 +105,11 @@ __device__ __forceinline__ void a8_split(const float (&x)[8], a8_frag (&to)[PIEC
             }
         }
     }
+}
+
+// Where the shares of a row are, in rows of the room: of a step in which few rows stand beside portions there is room for those few alone.
+__device__ __forceinline__ size_t a8_place(const A8Args& a, int seq, int kvh, int row, size_t out_row) {
+    return a.rows_each > 0 ? (static_cast<size_t>(seq) * a.nkv + kvh) * a.rows_each + row : out_row;
 }
 
 // Whether keys are more than the caller's longest context has.
@@ -521,7 +527,7 @@ __global__ __launch_bounds__(A8_WAVES * PL_WAVE, (A8Few<PIECES, DQ>::WAVES(RB)))
             __syncthreads();
         }
         if (wave == 0 && out_row[b] >= 0) {
-            const size_t place = static_cast<size_t>(out_row[b]) * a.parts + share;
+            const size_t place = a8_place(a, seq, kvh, 16 * b + col, out_row[b]) * a.parts + share;
             if (whole_row) {
                 if (!BALANCED && shares > 1) total = NAN;          // (a context longer than the caller said)
                 const float inv = total != 0.f ? 1.f / total : 0.f;
@@ -856,8 +862,8 @@ __global__ __launch_bounds__(A8_WAVES * PL_WAVE) void attention_8bit_merge_kerne
     for (int r = threadIdx.x / PL_WAVE + A8_WAVES * (block % every); r < rows; r += waves) {
         const int row = first_row + r;
         const size_t out_row = static_cast<size_t>(a.q_start[seq] + row / group) * a.nq + kvh * group + row % group;
-        const float* ml = a.part_ml + 2 * out_row * a.parts;
-        const float* acc = a.part_acc + out_row * a.parts * a.d;
+        const size_t place = a8_place(a, seq, kvh, row, out_row) * a.parts;
+        const float *ml = a.part_ml + 2 * place, *acc = a.part_acc + place * a.d;
         float top = -INFINITY, total = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
         const int at = 4 * (lane % lanes), from_at = min(at, a.d - 4);
         for (int base = 0; base < shares; base += PL_WAVE) {
@@ -1022,7 +1028,40 @@ extern "C" int pl_paged_attention_8bit_few(int d, int dtype) {
     return 16 * (dq <= 2 ? A8Few<1, 2>::BLOCKS : A8Few<1, 3>::BLOCKS);
 }
 
-// The kernel of few rows and that of many have shares of their own size.  Where either has more than one: `part_acc` has room for d floats for each of them (the larger number) and each of the n * nq rows,
+// Which kernels a step needs and what room their shares take, in rows of d values (and two numbers more): nothing for a kernel that does not run or has one share.
+struct A8Plan {
+    bool few_runs, many_runs;
+    int few;                  // a request's rows (tokens times query heads a key head) that the kernel of few takes, at most
+    int rows, rows_each;      // and may bring; A8Args::rows_each
+    long few_places, many_places;
+};
+static A8Plan a8_plan(int S, int n, int max_q_len, int min_q_len, int nq, int nkv, int d, int few_chunks, int many_chunks, int dtype) {
+    const long group = nq / nkv, longest = max_q_len * group, all = static_cast<long>(n) * nq;
+    A8Plan p{};
+    // In a step of portions only what 16 rows hold goes to the kernel of few: those are the single tokens beside them, for which its smallest form is the fastest
+    // (15 single tokens at up to 4,600 keys beside a portion: 32 us with it, 91 with the form for 64 rows).
+    p.few = pl_paged_attention_8bit_few(d, dtype);
+    p.many_runs = longest > p.few;
+    if (p.many_runs) p.few = 16;
+    p.few_runs = min_q_len * group <= p.few;
+    p.rows = static_cast<int>(longest < p.few ? longest : p.few);
+    // (as many as the build for so many rows holds: a request that brings more than it was said to stays inside its own)
+    const int held = pl_ceil_div(p.rows, 16) * 16;
+    const long each = static_cast<long>(S) * nkv * held;
+    if (each < all) p.rows_each = held;
+    if (p.few_runs && few_chunks > 1) p.few_places = (each < all ? each : all) * few_chunks;
+    if (p.many_runs && many_chunks > 1) p.many_places = all * many_chunks;
+    return p;
+}
+
+// How many rows of room pl_paged_attention_8bit needs for a step's shares.
+extern "C" long long pl_paged_attention_8bit_places(int S, int n, int max_q_len, int min_q_len, int nq, int nkv, int d, int few_chunks, int many_chunks, int dtype) {
+    if (nkv < 1 || nq < nkv || d < 1) return 0;
+    const A8Plan plan = a8_plan(S, n, max_q_len, min_q_len, nq, nkv, d, few_chunks, many_chunks, dtype);
+    return plan.few_places + plan.many_places;
+}
+
+// The kernel of few rows and that of many have shares of their own size.  `part_acc` has room for d floats for each of pl_paged_attention_8bit_places(...), those of many rows first;
 // `part_ml` for two, and for S more behind those.
 extern "C" int pl_paged_attention_8bit(const void* q, int q_stride, void* out, const void* q_start, const void* q_len, const void* ctx_len, int S, int n, int max_q_len, int min_q_len,
                                        const void* table, int width, int block, int pool_rows, const void* k_pool, const void* v_pool, const void* k_scale,
@@ -1033,34 +1072,35 @@ extern "C" int pl_paged_attention_8bit(const void* q, int q_stride, void* out, c
     PL_REQUIRE(S >= 1 && n >= 1 && max_q_len >= 1 && min_q_len <= max_q_len && width >= 1 && block >= 1 && pool_rows >= block,
                "8-bit attention: %d requests, %d rows, %d to %d of one request, tables of %d pages of %d, %d rows", S, n, min_q_len, max_q_len, width, block, pool_rows);
     PL_REQUIRE(static_cast<long>(n) * nq < (1l << 31) && (static_cast<long>(S) + 8) * nkv < (1l << 31), "8-bit attention: %d rows of %d heads, %d requests are too many for a launch", n, nq, S);
-    PL_REQUIRE(few_chunk >= A8_KEYS && few_chunk % A8_KEYS == 0 && few_chunk <= A8_MOST_KEYS && few_chunks >= 1 && few_chunks < 65536 && (few_chunks == 1 || (part_acc && part_ml)),
+    PL_REQUIRE(few_chunk >= A8_KEYS && few_chunk % A8_KEYS == 0 && few_chunk <= A8_MOST_KEYS && few_chunks >= 1 && few_chunks < 65536,
                "8-bit attention: %d shares of %d keys", few_chunks, few_chunk);
-    PL_REQUIRE(many_chunk >= 64 && many_chunk % 64 == 0 && many_chunks >= 1 && many_chunks < 65536 && (many_chunks == 1 || (part_acc && part_ml)),
+    PL_REQUIRE(many_chunk >= 64 && many_chunk % 64 == 0 && many_chunks >= 1 && many_chunks < 65536,
                "8-bit attention: %d shares of %d keys", many_chunks, many_chunk);
+    const A8Plan plan = a8_plan(S, n, max_q_len, min_q_len, nq, nkv, d, few_chunks, many_chunks, dtype);
+    PL_REQUIRE(plan.few_places + plan.many_places == 0 || (part_acc && part_ml), "8-bit attention: no room for %ld rows of shares", plan.few_places + plan.many_places);
     const int shift = 31 + (block > 1 ? 32 - __builtin_clz(block - 1) : 0);
     const uint32_t magic = static_cast<uint32_t>(((uint64_t{1} << shift) + block - 1) / block);
     A8Args a{q, q_stride, out, static_cast<const int*>(q_start), static_cast<const int*>(q_len), static_cast<const int*>(ctx_len), S, static_cast<const int*>(table), width, block, magic, shift, pool_rows / block,
              static_cast<const uint8_t*>(k_pool), static_cast<const uint8_t*>(v_pool), static_cast<const uint8_t*>(k_scale), static_cast<const uint8_t*>(v_scale),
-             nq, nkv, d, a8_beside(nkv, d), scale * 1.4426950408889634f, window, n, few_chunk, few_chunks, few_chunk, 0, static_cast<float*>(part_acc), static_cast<float*>(part_ml), max(few_chunks, many_chunks), nullptr};
-    if (part_ml) a.cut = reinterpret_cast<int*>(a.part_ml + 2l * n * nq * a.parts);
-    const long group = nq / nkv, longest = max_q_len * group;
-    // In a step of portions only what 16 rows hold goes to the kernel of few: those are the single tokens beside them, for which its smallest form is the fastest
-    // (15 single tokens at up to 4,600 keys beside a portion: 32 us with it, 91 with the form for 64 rows).
-    int few = pl_paged_attention_8bit_few(d, dtype);
-    if (longest > few) few = 16;
+             nq, nkv, d, a8_beside(nkv, d), scale * 1.4426950408889634f, window, n, few_chunk, few_chunks, few_chunk, 0, static_cast<float*>(part_acc), static_cast<float*>(part_ml), few_chunks, 0, nullptr};
     const hipStream_t on = static_cast<hipStream_t>(stream);
     const bool f32 = dtype == PL_DTYPE_F32;
-    A8Merge merge{a, a, 0, 0, 1, 1, few, 0};
+    A8Merge merge{a, a, 0, 0, 1, 1, plan.few, 0};
     long groups = 0;
-    if (min_q_len * group <= few) {
-        const int rows = static_cast<int>(min(longest, static_cast<long>(few)));
-        if (int e = f32 ? launch_few<3>(merge.few, rows, merge, on) : launch_few<1>(merge.few, rows, merge, on)) return e;
+    if (plan.few_runs) {
+        merge.few.rows_each = plan.rows_each;
+        if (plan.few_places > 0) {
+            merge.few.part_acc += plan.many_places * d;
+            merge.few.part_ml += plan.many_places * 2;
+            merge.few.cut = reinterpret_cast<int*>(merge.few.part_ml + plan.few_places * 2);
+        }
+        if (int e = f32 ? launch_few<3>(merge.few, plan.rows, merge, on) : launch_few<1>(merge.few, plan.rows, merge, on)) return e;
         if (few_chunks > 1) groups = static_cast<long>(S) * nkv * merge.few_groups;
     }
-    if (longest > few) {
+    if (plan.many_runs) {
         merge.many.chunk = many_chunk;
-        merge.many.chunks = many_chunks;
-        if (int e = f32 ? launch_many<3>(merge.many, few, max_q_len, merge, on) : launch_many<1>(merge.many, few, max_q_len, merge, on)) return e;
+        merge.many.chunks = merge.many.parts = many_chunks;
+        if (int e = f32 ? launch_many<3>(merge.many, plan.few, max_q_len, merge, on) : launch_many<1>(merge.many, plan.few, max_q_len, merge, on)) return e;
         groups += merge.tall;
     }
     if (groups == 0) return 0;

@@ -125,12 +125,14 @@ def _signatures(lib) -> None:
         "pl_qk_norm_rope_kv_write_8bit": [p, p, i, p, p, i, f, p, p, i, i, i, p, p, i, i, p, p, p, p, i, i, i, i, i, p],
         "pl_paged_attention_8bit": [p, i, p, p, p, p, i, i, i, i, p, i, i, i, p, p, p, p, i, i, i, f, i, i, i, i, i, p, p, i, p],
         "pl_paged_attention_8bit_few": [i, i],
+        "pl_paged_attention_8bit_places": [i, i, i, i, i, i, i, i, i, i],
         "pl_bigram_add": [p, p, p, p, p, p, p, p, p, p, p, i, ctypes.c_longlong, ctypes.c_longlong, ctypes.c_longlong, i, i, p],
     }
     for name, argtypes in table.items():
         fn = getattr(lib, name)
         fn.argtypes = argtypes
         fn.restype = c_int
+    lib.pl_paged_attention_8bit_places.restype = ctypes.c_longlong
 
 
 def library():
@@ -3084,6 +3086,14 @@ def shares_8bit(n: int, requests: int, max_ctx: int, nq: int, nkv: int, window: 
     return few + of((reach + 64 * shares - 1) // (64 * shares) * 64 if shares > 1 else (max_ctx + 63) // 64 * 64, reach)
 
 
+@functools.lru_cache(maxsize=4096)
+def _plan_8bit(n: int, requests: int, max_q_len: int, min_q_len: int, max_ctx: int, nq: int, nkv: int, window: int, d: int, code: int) -> tuple:
+    """``shares_8bit`` of a step, and how many rows of 32-bit results (d values and two more) the shares of the kernels that it runs leave to be put together: the many
+    rows' shares, at most some 33 MB at heads of 128, and for each request and key head those of its few rows (64 at most, 16 beside portions), a row for 2,048 keys of a long context."""
+    cut = shares_8bit(n, requests, max_ctx, nq, nkv, window, d, code == F32)
+    return cut + (library().pl_paged_attention_8bit_places(requests, n, max_q_len, min_q_len, nq, nkv, d, cut[1], cut[3], code),)
+
+
 def paged_attention_8bit(q: torch.Tensor, q_row_stride: int, out: torch.Tensor, q_start: torch.Tensor, q_len: torch.Tensor, ctx_len: torch.Tensor, max_q_len: int,
                          max_ctx: int, block_table: torch.Tensor, block_size: int, k_pool: torch.Tensor, v_pool: torch.Tensor, k_scale: torch.Tensor,
                          v_scale: torch.Tensor, nq: int, nkv: int, d: int, scale: float, window: int = 0, min_q_len: int = 1) -> torch.Tensor:
@@ -3114,13 +3124,12 @@ def paged_attention_8bit(q: torch.Tensor, q_row_stride: int, out: torch.Tensor, 
     queries, results = _fits(q, "query buffer", q.dtype, n * q_row_stride, device), _fits(out, "attention output", q.dtype, n * nq * d, device, (n, nq * d))
     if q_row_stride % 8 or (queries | results) % 16:
         raise TensorError("query rows and outputs for an 8-bit cache begin at whole 16 bytes")
-    few, few_shares, many, many_shares = shares_8bit(n, S, max_ctx, nq, nkv, window, d, code == F32)
-    chunks = max(few_shares, many_shares)
+    few, few_shares, many, many_shares, places = _plan_8bit(n, S, max_q_len, min_q_len, max_ctx, nq, nkv, window, d, code)
     acc = ml = 0
-    if chunks > 1:
-        room = torch.empty(n * nq * chunks * (d + 2) + S, dtype=torch.float32, device=q.device)
+    if places > 0:
+        room = torch.empty(places * (d + 2) + S, dtype=torch.float32, device=q.device)
         acc = room.data_ptr()
-        ml = acc + 4 * n * nq * chunks * d
+        ml = acc + 4 * places * d
     _check(library().pl_paged_attention_8bit(
         queries, q_row_stride, results, _fits(q_start, "first row of each request", torch.int32, S, device), _fits(q_len, "tokens of each request", torch.int32, S, device),
         _fits(ctx_len, "context length of each request", torch.int32, S, device), S, n, max_q_len, min_q_len, _fits(block_table, "block table", torch.int32, S * width, device), width,
