@@ -999,12 +999,15 @@ static int launch_many_blocks(const A8Args& a, int few, int max_q_len, A8Merge& 
 
 // Four waves a workgroup where eight's registers or LDS leave no second one beside it anyway (32 bits, heads of more than 128) or where two of four fit a unit (heads of up to 64: 2 prompts of 1,500 to 2,000 tokens,
 // 16 heads over 8, 45 us with eight, 40 with four); else eight, which widen a tile for 256 rows, but for so few rows that workgroups of 128 do not fill the chip either (512 tokens of 16 heads over 8: 23.5 and 20.8 us).
+static int a8_waves(int n, int nq, int nkv, int d, int chunks, int dtype) {
+    const long blocks = (static_cast<long>(n) * (nq / nkv) + 127) / 128 * nkv * chunks;
+    return dtype == PL_DTYPE_BF16 && d > 64 && d <= 128 && blocks > 256 ? 8 : 4;
+}
+
 template <int PIECES, int DT>
 static int launch_many(const A8Args& a, int few, int max_q_len, A8Merge& merge, hipStream_t stream) {
-    if constexpr (PIECES == 1 && (DT == 3 || DT == 4)) {
-        const long blocks = (static_cast<long>(a.n) * (a.nq / a.nkv) + 127) / 128 * a.nkv * a.chunks;
-        if (blocks > 256) return launch_many_blocks<PIECES, DT, 8>(a, few, max_q_len, merge, stream);
-    }
+    if constexpr (PIECES == 1 && (DT == 3 || DT == 4))
+        if (a8_waves(a.n, a.nq, a.nkv, a.d, a.chunks, PL_DTYPE_BF16) == 8) return launch_many_blocks<PIECES, DT, 8>(a, few, max_q_len, merge, stream);
     return launch_many_blocks<PIECES, DT, 4>(a, few, max_q_len, merge, stream);
 }
 
@@ -1027,6 +1030,9 @@ extern "C" int pl_paged_attention_8bit_few(int d, int dtype) {
     if (dtype == PL_DTYPE_F32) return 16 * (dq == 1 ? A8Few<3, 1>::BLOCKS : dq == 2 ? A8Few<3, 2>::BLOCKS : A8Few<3, 3>::BLOCKS);
     return 16 * (dq <= 2 ? A8Few<1, 2>::BLOCKS : A8Few<1, 3>::BLOCKS);
 }
+
+// The waves of a workgroup of the kernel of many rows, for `chunks` shares.
+extern "C" int pl_paged_attention_8bit_waves(int n, int nq, int nkv, int d, int chunks, int dtype) { return nkv >= 1 ? a8_waves(n, nq, nkv, d, chunks, dtype) : 0; }
 
 // Which kernels a step needs and what room their shares take, in rows of d values (and two numbers more): nothing for a kernel that does not run or has one share.
 struct A8Plan {
