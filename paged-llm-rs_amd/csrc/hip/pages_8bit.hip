@@ -415,15 +415,30 @@ __global__ __launch_bounds__(P8_WAVES * PL_WAVE) void write_8bit_kernel(P8Write 
     }
 }
 
-template <typename T, int LPR>
-static int launch_write(const P8Write& a, hipStream_t stream) {
-    constexpr int ROWS = P8_WAVES * PL_WAVE / LPR;
+// Lanes a row of d values, eight each.
+static int p8_lanes(int d) { return d <= 32 ? 4 : d <= 64 ? 8 : d <= 128 ? 16 : 32; }
+
+// How a step is written: the rows that a wave looks through for the first ones of runs, and the waves that take a run.
+struct P8Shape {
+    int tile, waves;
+};
+static P8Shape p8_shape(int n, int nkv, int block, int d) {
     // A wave takes a run, 64 / LPR rows at a time; in steps of many rows a workgroup does, four times as many.  It looks through `tile` rows for the first ones of runs: one each while all of a
     // step's may be first (decoding), else 32, since most of many rows are inside a page, and units that find nothing still cost their start: 10,503 rows of prompts into 8 heads take 182 us with a
     // workgroup a row and 77 with 32 rows, 600 single tokens 30 us with a workgroup each and 14 with a wave.  (Values of more rows held in registers, so that a run is not read again from L2 once its
     // power is known, cost the queries' workgroups of the same launch their places: 94 us with twice the rows, 117 with four times.)
-    const int tile = static_cast<long>(a.n) * 2 * a.nkv <= P8_SINGLE_UNITS ? 1 : 32;
-    const bool whole = tile > 1 && a.block > PL_WAVE / LPR;
+    const int tile = static_cast<long>(n) * 2 * nkv <= P8_SINGLE_UNITS ? 1 : 32;
+    return P8Shape{tile, tile > 1 && block > PL_WAVE / p8_lanes(d) ? P8_WAVES : 1};
+}
+extern "C" int pl_qk_norm_rope_kv_write_8bit_tile(int n, int nkv, int block, int d) { return p8_shape(n, nkv, block, d).tile; }
+extern "C" int pl_qk_norm_rope_kv_write_8bit_waves(int n, int nkv, int block, int d) { return p8_shape(n, nkv, block, d).waves; }
+
+template <typename T, int LPR>
+static int launch_write(const P8Write& a, hipStream_t stream) {
+    constexpr int ROWS = P8_WAVES * PL_WAVE / LPR;
+    const P8Shape shape = p8_shape(a.n, a.nkv, a.block, a.d);
+    const int tile = shape.tile;
+    const bool whole = shape.waves > 1;
     const long units = a.slots != nullptr ? static_cast<long>(pl_ceil_div(a.n, tile)) * 2 * a.nkv : 0;
     const long groups = (whole ? units : (units + P8_WAVES - 1) / P8_WAVES) + (static_cast<long>(a.n) * pl_ceil_div(a.nq, P8_HEADS) + ROWS - 1) / ROWS;
     PL_REQUIRE(groups < (1l << 31) && static_cast<long>(a.n) * a.nq < (1l << 31) - ROWS, "8-bit write: %d rows of %d heads are too many for a launch", a.n, a.nq + 2 * a.nkv);
@@ -437,10 +452,12 @@ static int launch_write(const P8Write& a, hipStream_t stream) {
 
 template <typename T>
 static int launch_write(const P8Write& a, hipStream_t stream) {
-    if (a.d <= 32) return launch_write<T, 4>(a, stream);
-    if (a.d <= 64) return launch_write<T, 8>(a, stream);
-    if (a.d <= 128) return launch_write<T, 16>(a, stream);
-    return launch_write<T, 32>(a, stream);
+    switch (p8_lanes(a.d)) {
+        case 4: return launch_write<T, 4>(a, stream);
+        case 8: return launch_write<T, 8>(a, stream);
+        case 16: return launch_write<T, 16>(a, stream);
+        default: return launch_write<T, 32>(a, stream);
+    }
 }
 
 extern "C" int pl_qk_norm_rope_kv_write_8bit(const void* qkv, void* q, int q_stride, const void* q_gain, const void* k_gain, int gain_dtype, float eps, const void* cos,

@@ -126,6 +126,8 @@ def _signatures(lib) -> None:
         "pl_paged_attention_8bit": [p, i, p, p, p, p, i, i, i, i, p, i, i, i, p, p, p, p, i, i, i, f, i, i, i, i, i, p, p, i, p],
         "pl_paged_attention_8bit_few": [i, i],
         "pl_paged_attention_8bit_waves": [i, i, i, i, i, i],
+        "pl_qk_norm_rope_kv_write_8bit_tile": [i, i, i, i],
+        "pl_qk_norm_rope_kv_write_8bit_waves": [i, i, i, i],
         "pl_paged_attention_8bit_places": [i, i, i, i, i, i, i, i, i, i],
         "pl_bigram_add": [p, p, p, p, p, p, p, p, p, p, p, i, ctypes.c_longlong, ctypes.c_longlong, ctypes.c_longlong, i, i, p],
     }

@@ -64,3 +64,107 @@ def test_many_rows_with_eight_waves_a_workgroup(nq, nkv, d, requests, window):
     if len(requests) == 16 and nq // nkv == 2 and window == 0:
         assert shares > 1
     scene.check(scene.run(window, min_q_len=0), window)
+
+
+# ---- the write of many rows ----------------------------------------------------------------------------------------------
+
+def least_power(top):
+    """The bytes of the least powers of two whose 448-fold holds ``top`` (64-bit, not negative)."""
+    part, exponent = torch.frexp(top)
+    return torch.where(top > 0, exponent - 9 + (part > 0.875).int(), torch.full_like(exponent, -126)).clamp(min=-126) + 127
+
+
+def plain_write(pages, which, rows, slots, slack):
+    """What the pools ought to hold and the least and largest power of every page and head: ``rows`` [n, nkv, d] in 64 bits, ``slots`` a list (-1: nowhere), values known to within
+    ``slack`` of themselves.  (values in 64 bits before their rounding, which slots they are in, least power, largest power, pages written)"""
+    block = pages.block
+    live = torch.tensor([r for r, s in enumerate(slots) if s >= 0], device=rows.device)
+    at = torch.tensor([s for s in slots if s >= 0], device=rows.device)
+    page = at // block
+    # a page is begun anew where its first slot is among those written
+    first = torch.full((pages.powers[which].shape[0],), block, device=rows.device, dtype=torch.long).scatter_reduce_(0, page, at % block, "amin")
+    top = torch.zeros(pages.powers[which].shape, dtype=torch.float64, device=rows.device).index_reduce_(0, page, rows[live].abs().amax(-1), "amax")
+    had = torch.where(((first > 0) & (first < block)).view(-1, 1), pages.powers[which].view(torch.uint8).int(), torch.zeros_like(pages.powers[which].view(torch.uint8).int()))
+    return at, live, page, first, torch.maximum(least_power(top * (1 - slack)), had), torch.maximum(least_power(top * (1 + slack)), had)
+
+
+def check_write(pages, before, which, rows, slots, exact):
+    """``exact``: the values took no arithmetic on the way, so powers and bytes are those of the definition.  Else they are off by at most 1e-5 of the row's largest before the rounding (32-bit norms
+    and rotations), so a maximum near a border may fall on either side, and a byte is off by half a step of e4m3 beside that."""
+    block, nkv, d = pages.block, pages.nkv, pages.d
+    at, live, page, first, least, most = plain_write(before, which, rows, slots, 0.0 if exact else 1e-5)
+    got, was = (p.powers[which].view(torch.uint8).int() for p in (pages, before))
+    written = first < block
+    assert torch.equal(got[~written], was[~written])
+    assert bool(((got >= least) & (got <= most))[written].all())
+    unit = torch.exp2(got.double() - 127)
+    held, then = (p.pools[which].double().view(-1, nkv, d) for p in (pages, before))
+    want = rows[live]
+    u = unit[page].unsqueeze(-1)
+    if exact:
+        assert torch.equal(pages.pools[which].view(-1, nkv, d)[at].view(torch.uint8), (want / u).float().to(cache.E4M3).view(torch.uint8))
+    off = (held[at] * u - want).abs()
+    assert bool((off <= torch.maximum(cache.HALF_E4M3 * want.abs(), 2.0 ** -10 * u) + (0 if exact else 1e-5) * want.abs().amax(-1, keepdim=True)).all())
+    # what was there in front of a page's new rows: as it was, or rounded again in the new unit, to the bit
+    place = torch.arange(held.shape[0], device=held.device)
+    kept = written[place // block] & (place % block < first[place // block])
+    # (nearest, ties to even, of what a power of two divides exactly)
+    fewer = torch.exp2((was - got).double())[place // block].unsqueeze(-1)
+    assert torch.equal(pages.pools[which].view(-1, nkv, d)[kept].view(torch.uint8), (then * fewer)[kept].float().to(cache.E4M3).view(torch.uint8))
+    touched = torch.zeros(held.shape[0], dtype=torch.bool, device=held.device)
+    touched[at] = True
+    same = ~(touched | kept)
+    assert torch.equal(pages.pools[which].view(torch.uint8)[same], before.pools[which].view(torch.uint8)[same])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("nq,nkv,d,block,rot,normed,neighbours,waves", [
+    (16, 8, 128, 16, 128, True, False, 4), (16, 8, 128, 5, 128, True, False, 4), (16, 8, 128, 3, 128, True, False, 1), (8, 8, 128, 128, 64, False, False, 4), (4, 8, 64, 16, 64, True, False, 4),
+    (4, 8, 64, 8, 30, True, False, 1), (4, 8, 96, 300, 90, True, False, 4), (8, 8, 256, 16, 256, True, False, 4), (8, 8, 256, 2, 0, True, False, 1), (12, 12, 32, 32, 32, False, True, 4),
+    (0, 12, 16, 16, 0, False, False, 1), (8, 8, 176, 1, 22, True, True, 1)])
+def test_many_rows_into_their_pages(dtype, nq, nkv, d, block, rot, normed, neighbours, waves):
+    """Steps of enough rows to be looked through 32 at a time, a wave or four to a run: prompts that end inside such a tile, requests that begin inside a page whose power grows or does not, runs that
+    cross tiles, several runs a tile, rows of padding between."""
+    from paged_llm_rs_amd import kernels
+
+    lens = [(0, 700), (7, 3), (block // 2, 260), (0, 1), (block - 1, 2), (3 * block + 1, 95), (0, 33), (0, 31), (0, block), (block // 3, 4)]      # (tokens there already, tokens that come)
+    need = [cache.pages_of(a + b, block) for a, b in lens]
+    order = torch.randperm(sum(need) + 5).tolist()
+    slots, positions = [], []
+    for s, (there, comes) in enumerate(lens):
+        mine = order[sum(need[:s]):sum(need[:s + 1])]
+        slots += [mine[p // block] * block + p % block for p in range(there, there + comes)]
+        positions += list(range(there, there + comes))
+        if s % 3 == 1:
+            slots += [-1] * (5 + s)
+            positions += [-1] * (5 + s)
+    n = len(slots)
+    lib = kernels.library()
+    assert lib.pl_qk_norm_rope_kv_write_8bit_tile(n, nkv, block, d) == 32 and lib.pl_qk_norm_rope_kv_write_8bit_waves(n, nkv, block, d) == waves
+    qkv = (torch.randn(n, (nq + 2 * nkv) * d, device=cache.DEV) * torch.exp2(3 * torch.randn(n, 1, device=cache.DEV)) * torch.exp2(2 * torch.randn(n, (nq + 2 * nkv) * d, device=cache.DEV))).to(dtype)
+    gains = tuple((1 + 0.3 * torch.randn(d, device=cache.DEV)).to(dtype) for _ in range(2)) if normed else (None, None)
+    angle = torch.rand(max(positions) + 1, max(rot // 2, 1), device=cache.DEV) * 6
+    cos, sin = angle.cos(), angle.sin()
+    pages = cache.Pages(len(order), block, nkv, d)
+    for pool, power in zip(pages.pools, pages.powers):       # (what earlier steps left: some pages keep their power, some do not)
+        pool.copy_((torch.randn(pool.shape, device=cache.DEV) * 60).clamp(-448, 448).to(cache.E4M3))
+        power.view(torch.uint8).copy_(torch.randint(112, 130, power.shape, device=cache.DEV))
+    before = pages.clone()
+    q = torch.full((n, nq * d), -5.0, dtype=dtype, device=cache.DEV)
+    at = cache.i32(positions)
+    cache.write(pages, qkv, cache.i32(slots), at, nq, q=q, gains=gains, cos=cos, sin=sin, rot=rot, neighbours=neighbours)
+    x = qkv.double().view(n, nq + 2 * nkv, d)
+    keys = cache.plain_heads(x[:, nq:nq + nkv], gains[1], 1e-6, cos, sin, rot, at, neighbours)
+    check_write(pages, before, 0, keys, slots, not normed and not rot)
+    check_write(pages, before, 1, x[:, nq + nkv:], slots, True)
+    live = at >= 0
+    assert bool((q[~live] == -5).all())
+    if nq:
+        want = cache.plain_heads(x[:, :nq], gains[0], 1e-6, cos, sin, rot, at, neighbours).reshape(n, nq * d)
+        allowed = (cache.HALF_BF16 if dtype == torch.bfloat16 else 0) * want.abs() + 1e-5 * want.abs().view(n, nq, d).amax(-1, keepdim=True).expand(n, nq, d).reshape(n, -1)
+        assert bool(((q.double() - want).abs() <= allowed)[live].all())
+    # in place
+    twin, again = before.clone(), qkv.clone()
+    cache.write(twin, again, cache.i32(slots), at, nq, gains=gains, cos=cos, sin=sin, rot=rot, neighbours=neighbours)
+    assert torch.equal(again[live, :nq * d], q[live]) and torch.equal(again[:, nq * d:], qkv[:, nq * d:]) and torch.equal(again[~live], qkv[~live])
+    assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(twin, pages))
