@@ -168,3 +168,15 @@ def test_many_rows_into_their_pages(dtype, nq, nkv, d, block, rot, normed, neigh
     cache.write(twin, again, cache.i32(slots), at, nq, gains=gains, cos=cos, sin=sin, rot=rot, neighbours=neighbours)
     assert torch.equal(again[live, :nq * d], q[live]) and torch.equal(again[:, nq * d:], qkv[:, nq * d:]) and torch.equal(again[~live], qkv[~live])
     assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(twin, pages))
+
+
+def test_the_most_requests_of_a_step():
+    """8,192 requests, which take all the room that the kernel has for their sums, with pages from a list of free ones and without."""
+    requests = 8192
+    ctx = [1 + (7 * s) % 50 for s in range(requests)]
+    q_len = [c if s % 5 == 0 else 1 for s, c in enumerate(ctx)]
+    ctx[17], q_len[17] = 0, 3
+    table = [[4 * s + i for i in range(4)] for s in range(requests)]
+    free = list(range(4 * requests, 4 * requests + 9000))
+    cache.check_tables(q_len, ctx, table, 16, free, sum(q_len) + 11)
+    cache.check_tables(q_len, ctx, table, 16, None, sum(q_len) + 11)
