@@ -257,6 +257,75 @@ __device__ __forceinline__ float a8_max_quarters(float v) {
     return fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1]));
 }
 
+// ---- a row by itself ----------------------------------------------------------------------------------------------------
+// A weight of zero does not hide a value that is not finite, and a tile's values meet the rows of several tokens, which need not all see its keys.  So where the rows of a workgroup do not all see its keys,
+// and a row's result is not finite, a wave works that row out again from the keys [lo, hi) that it sees, one by one, and the row is what these make it.  (Looking at every tile's values among the work on it
+// cost 2 to 15%, whether or not there are any.)
+// A function that is called, and that reads the launch's arguments anew: worked into the kernels it takes registers from their loops (184 instead of 148 for single tokens, a third of their workgroups).
+__device__ __forceinline__ const A8Args& a8_args_again() {
+    uint64_t at = reinterpret_cast<uint64_t>(__builtin_amdgcn_kernarg_segment_ptr());          // (their first argument in both)
+    asm volatile("" : "+s"(at));
+    return *reinterpret_cast<const A8Args*>(at);
+}
+template <int PIECES>
+__device__ __attribute__((noinline)) void a8_row_alone(const A8Args& a, int seq, int kvh, int lo, int hi, size_t row, size_t place, bool whole, int head) {
+    typedef typename A8Type<PIECES>::type T;
+    const int lane = threadIdx.x % PL_WAVE;
+    const T* q = static_cast<const T*>(a.q) + row * a.q_stride + static_cast<size_t>(head) * a.d;
+    float m = -INFINITY, l = 0.f, out[4] = {0.f, 0.f, 0.f, 0.f};         // the columns lane, lane + 64, ...
+#pragma unroll 1
+    for (int base = lo; base < hi; base += PL_WAVE) {
+        const int key = min(base + lane, hi - 1), index = a8_page_index(a, key);
+        const int found = a.table[static_cast<size_t>(seq) * a.width + min(index, a.width - 1)];
+        const int page = static_cast<unsigned>(found) < static_cast<unsigned>(a.pages) ? found : 0, slot = page * a.block + key - index * a.block;
+        const size_t at = (static_cast<size_t>(slot) * a.nkv + kvh) * a.d, power = static_cast<size_t>(page) * a.nkv + kvh;
+        float score = 0.f;
+#pragma unroll 1
+        for (int c = 0; c < a.d; c += 4) {
+            const uint32_t bytes = *reinterpret_cast<const uint32_t*>(a.k_pool + at + c);
+            const a8_f32x2 k01 = __builtin_amdgcn_cvt_pk_f32_fp8(bytes, false), k23 = __builtin_amdgcn_cvt_pk_f32_fp8(bytes, true);
+            score = fmaf(to_float(q[c]), k01[0], fmaf(to_float(q[c + 1]), k01[1], fmaf(to_float(q[c + 2]), k23[0], fmaf(to_float(q[c + 3]), k23[1], score))));
+        }
+        score = base + lane < hi ? score * a8_unit(a.k_scale[power]) * a.scale : -INFINITY;
+        const float grown = fmaxf(m, wave_max(score)), from = grown == -INFINITY ? 0.f : grown;
+        const float alpha = __builtin_amdgcn_exp2f(m - from), weight = __builtin_amdgcn_exp2f(score - from);
+        const float unit = a8_unit(a.v_scale[power]);
+        m = grown;
+        l = l * alpha + weight;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) out[i] *= alpha;
+        const int here = min(hi - base, PL_WAVE);
+#pragma unroll 1
+        for (int eight = 0; eight < here; eight += 8) {                // (eight keys among themselves first: fewer roundings behind each other)
+            float x[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+            for (int j = eight; j < min(eight + 8, here); ++j) {
+                const float w = __shfl(weight, j, PL_WAVE), u = __shfl(unit, j, PL_WAVE);
+                const uint8_t* v = a.v_pool + (static_cast<size_t>(__shfl(slot, j, PL_WAVE)) * a.nkv + kvh) * a.d;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (lane + PL_WAVE * i < a.d) x[i] = fmaf(w, __builtin_amdgcn_cvt_f32_fp8(v[lane + PL_WAVE * i], 0) * u, x[i]);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) out[i] += x[i];
+        }
+    }
+    l = wave_sum(l);
+    const size_t out_row = row * a.nq + head;
+    const float inv = l != 0.f ? 1.f / l : 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int c = lane + PL_WAVE * i;
+        if (c >= a.d) continue;
+        if (whole) static_cast<T*>(a.out)[out_row * a.d + c] = from_float<T>(out[i] * inv);
+        else a.part_acc[place * a.d + c] = out[i];
+    }
+    if (!whole && lane == 0) {
+        a.part_ml[2 * place] = m;
+        a.part_ml[2 * place + 1] = l;
+    }
+}
+
 // ---- few rows: every wave has keys of its own ------------------------------------------------------------------------------
 // A workgroup takes the RB blocks of 16 rows of one request and key head and one share of the keys; its waves take tiles of 32 keys in turn, each with a running maximum and sum, and meet at the end.
 // Keys go from memory into the registers that the product reads (a lane reads 16 bytes of one key: the contraction may go through a head's values in any order, so the
@@ -502,6 +571,9 @@ __global__ __launch_bounds__(A8_WAVES * PL_WAVE, (A8Few<PIECES, DQ>::WAVES(RB)))
         }
     }
     __syncthreads();
+    // (not all rows see all keys of the share)
+    const bool unlike = k_begin < last_from || k_end - 1 > start;
+    uint64_t again = 0;                          // rows that are worked out once more
     float* meet = reinterpret_cast<float*>(lds);
 #pragma unroll
     for (int b = 0; b < RB; ++b) {
@@ -527,6 +599,16 @@ __global__ __launch_bounds__(A8_WAVES * PL_WAVE, (A8Few<PIECES, DQ>::WAVES(RB)))
             __syncthreads();
         }
         if (wave == 0 && out_row[b] >= 0) {
+            if (unlike) {
+                float finite = 0.f;              // (or NaN)
+#pragma unroll
+                for (int t = 0; t < 4 * DQ; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) finite = fmaf(acc[b][t][i], 0.f, finite);
+                uint64_t bad = __ballot(finite != finite && total == total);          // (weights that are NaN leave nothing else)
+                bad |= bad >> 32;
+                again |= ((bad | bad >> 16) & 0xffff) << (16 * b);
+            }
             const size_t place = a8_place(a, seq, kvh, 16 * b + col, out_row[b]) * a.parts + share;
             if (whole_row) {
                 if (!BALANCED && shares > 1) total = NAN;          // (a context longer than the caller said)
@@ -546,6 +628,14 @@ __global__ __launch_bounds__(A8_WAVES * PL_WAVE, (A8Few<PIECES, DQ>::WAVES(RB)))
                 else *reinterpret_cast<a8_f32x4*>(a.part_acc + place * a.d + at) = acc[b][t];
             }
         }
+    }
+    again = static_cast<uint64_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(again >> 32))) << 32 | static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(again)));
+    if (again == 0 || wave != 0 || (!BALANCED && whole_row && shares > 1)) return;
+    __threadfence_block();
+    for (; again != 0; again &= again - 1) {
+        const int row = __ffsll(static_cast<unsigned long long>(again)) - 1, token = row / group, head = kvh * group + row % group;
+        const size_t place = a8_place(a, seq, kvh, row, static_cast<size_t>(q_start + token) * a.nq + head) * a.parts + share;
+        a8_row_alone<PIECES>(a8_args_again(), seq, kvh, max(pl_first_visible(start + token, a.window), k_begin), min(start + token + 1, k_end), q_start + token, place, whole_row, head);
     }
 }
 
@@ -802,26 +892,45 @@ __global__ __launch_bounds__(NW * PL_WAVE) __attribute__((amdgpu_waves_per_eu(A8
         if (t + 1 < tiles) round(s[1], s[0], t + 1);
     }
     l += __shfl_xor(l, 32, PL_WAVE);
-    if (!live) return;
+    uint32_t again = 0;                       // rows that are worked out once more
+    if (k_begin < last_from || k_end - 1 > first_pos) {          // (not all of the wave's rows see all keys of the share)
+        float finite = 0.f;                   // (or NaN)
+#pragma unroll
+        for (int t = 0; t < DT; ++t)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) finite = fmaf(acc[t][i], 0.f, finite);
+        const uint64_t bad = __ballot(live && finite != finite && l == l);          // (weights that are NaN leave nothing else)
+        again = static_cast<uint32_t>(bad | bad >> 32);
+    }
+    if (!active) return;
 
     const size_t out_row = static_cast<size_t>(q_start + token) * a.nq + head, place = out_row * a.parts + share;
-    float inv = 1.f;
-    if (a.chunks == 1) {
-        if (shares > 1) l = NAN;              // (a context longer than the caller said)
-        inv = l != 0.f ? 1.f / l : 0.f;
-    } else if (half == 0) {
-        a.part_ml[2 * place] = m;
-        a.part_ml[2 * place + 1] = l;
-    }
-#pragma unroll
-    for (int t = 0; t < DT; ++t)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int at = 32 * t + 8 * i + 4 * half;
-            if (at >= a.d) continue;
-            if (a.chunks == 1) a8_store4<PIECES>(a, out_row * a.d + at, acc[t][4 * i] * inv, acc[t][4 * i + 1] * inv, acc[t][4 * i + 2] * inv, acc[t][4 * i + 3] * inv);
-            else *reinterpret_cast<a8_f32x4*>(a.part_acc + place * a.d + at) = a8_f32x4{acc[t][4 * i], acc[t][4 * i + 1], acc[t][4 * i + 2], acc[t][4 * i + 3]};
+    if (live) {
+        float inv = 1.f;
+        if (a.chunks == 1) {
+            if (shares > 1) l = NAN;              // (a context longer than the caller said)
+            inv = l != 0.f ? 1.f / l : 0.f;
+        } else if (half == 0) {
+            a.part_ml[2 * place] = m;
+            a.part_ml[2 * place + 1] = l;
         }
+#pragma unroll
+        for (int t = 0; t < DT; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int at = 32 * t + 8 * i + 4 * half;
+                if (at >= a.d) continue;
+                if (a.chunks == 1) a8_store4<PIECES>(a, out_row * a.d + at, acc[t][4 * i] * inv, acc[t][4 * i + 1] * inv, acc[t][4 * i + 2] * inv, acc[t][4 * i + 3] * inv);
+                else *reinterpret_cast<a8_f32x4*>(a.part_acc + place * a.d + at) = a8_f32x4{acc[t][4 * i], acc[t][4 * i + 1], acc[t][4 * i + 2], acc[t][4 * i + 3]};
+            }
+    }
+    if (again == 0 || (a.chunks == 1 && shares > 1)) return;
+    __threadfence_block();
+    for (; again != 0; again &= again - 1) {
+        const int r = first_row + 32 * wave + __ffs(again) - 1, of = r / group, query = kvh * group + r % group;
+        a8_row_alone<PIECES>(a8_args_again(), seq, kvh, max(pl_first_visible(start + of, a.window), k_begin), min(start + of + 1, k_end), q_start + of,
+                             (static_cast<size_t>(q_start + of) * a.nq + query) * a.parts + share, a.chunks == 1, query);
+    }
 }
 
 // ---- shares put together ---------------------------------------------------------------------------------------------------

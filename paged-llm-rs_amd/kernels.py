@@ -3106,8 +3106,8 @@ def paged_attention_8bit(q: torch.Tensor, q_row_stride: int, out: torch.Tensor, 
     as they were in ``out``.
 
     ``max_q_len``, ``min_q_len`` and ``max_ctx`` bound what the requests bring and their contexts (the launches are sized and chosen by them): rows whose keys reach past ``max_ctx`` come out as NaN, and
-    rows past ``max_q_len`` of a request may be left out.  The caller answers for the pages of all keys that are seen; keys that no row of a request sees may hold anything
-    (a NaN among the values that some row sees may reach the other rows that its request brings)."""
+    rows past ``max_q_len`` of a request may be left out.  The caller answers for the pages of all keys that are seen; what a row does not see
+    may hold anything: a NaN there reaches the rows that see it and no other."""
     device = torch.cuda.current_device()
     max_q_len, min_q_len, max_ctx, window = int(max_q_len), int(min_q_len), int(max_ctx), int(window or 0)
     code = _code(q, "query buffer")
