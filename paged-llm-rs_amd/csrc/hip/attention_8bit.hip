@@ -773,14 +773,20 @@ __global__ __launch_bounds__(NW * PL_WAVE) __attribute__((amdgpu_waves_per_eu(A8
                 for (int p = PIECES - 1; p >= 0; --p) s[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf.vec, qf[j][p].vec, s[kb], 0, 0, 0);
             }
     };
+    // (Values are chosen under the branch and put back behind it, as in the kernel of few rows: see there.)
     auto mask = [&](a8_f32x16 (&s)[KB], int k0) {
+        float x[16 * KB];
 #pragma unroll
-        for (int kb = 0; kb < KB; ++kb)
+        for (int i = 0; i < 16 * KB; ++i) x[i] = s[i / 16][i % 16];
+        if (!whole(k0)) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const int key = k0 + 32 * kb + 8 * (i / 4) + 4 * half + i % 4;
-                s[kb][i] = static_cast<unsigned>(key - seen_from) < static_cast<unsigned>(seen) ? s[kb][i] : -INFINITY;
+            for (int i = 0; i < 16 * KB; ++i) {
+                const int key = k0 + 32 * (i / 16) + 8 * (i % 16 / 4) + 4 * half + i % 4;
+                x[i] = static_cast<unsigned>(key - seen_from) < static_cast<unsigned>(seen) ? x[i] : -INFINITY;
             }
+        }
+#pragma unroll
+        for (int i = 0; i < 16 * KB; ++i) s[i / 16][i % 16] = x[i];
     };
     auto largest = [&](const a8_f32x16 (&s)[KB]) {
         float most = s[0][0];
@@ -832,7 +838,7 @@ __global__ __launch_bounds__(NW * PL_WAVE) __attribute__((amdgpu_waves_per_eu(A8
             for (int g = 0; g < 2 * KB; ++g)
 #pragma unroll
                 for (int p = 0; p < PIECES; ++p) asm volatile("" : "+v"(pf[g][p].raw));
-            if (!whole(k0 + TILE)) mask(next, k0 + TILE);
+            mask(next, k0 + TILE);
             top = largest(next);
             const uint16_t* v_from = values + (v_now * TILE + 4 * half + lane % 16 / 4) * VROW + 16 * (lane / 16 % 2) + 4 * (lane % 4);
             // (In this order, AHEAD reads before the product that needs the first: left to itself the compiler waits for every pair of them.  Other instructions may move across.)
