@@ -2974,7 +2974,7 @@ def step_tables(q_len: torch.Tensor, ctx_len: torch.Tensor, block_table: torch.T
         raise TensorError(f"tokens of each request have shape {tuple(q_len.shape)}, expected [1 to {STEP_TABLES_MAX_SEQS}]")
     if block_table.dim() != 2 or block_table.shape[0] != S or block_table.shape[1] < 1:
         raise TensorError(f"block table has shape {tuple(block_table.shape)}, expected [{S}, pages]")
-    if rows < 0 or block_size < 1:
+    if not 0 <= rows < 2 ** 31 or not 1 <= block_size < 2 ** 31:
         raise TensorError(f"{rows} rows of pages of {block_size} tokens")
     width = block_table.shape[1]
     brings = _fits(q_len, "tokens of each request", torch.int32, S, device)
@@ -3037,12 +3037,16 @@ def qk_norm_rope_kv_write_8bit(qkv: torch.Tensor, q: torch.Tensor | None, q_gain
         q_gains, k_gains = _fits(q_gain, "query norm gain", q_gain.dtype, d, device), _fits(k_gain, "key norm gain", q_gain.dtype, d, device)
     cosines = sines = angles = 0
     if rot:
+        if cos is None or sin is None:
+            raise TensorError(f"a rotation over {rot} values of a head without its tables")
         if rot % 2 or not 0 < rot <= d or cos.dim() != 2 or cos.shape[1] != rot // 2 or cos.shape[0] < 1:
             raise TensorError(f"rotary tables have shape {tuple(cos.shape)}, expected [positions, {rot // 2}] for a rotation over {rot} values of a head of {d}")
         angles = cos.shape[0]
         cosines, sines = _fits(cos, "cosine table", torch.float32, angles * (rot // 2), device), _fits(sin, "sine table", torch.float32, angles * (rot // 2), device, cos.shape)
     if (source | queries | q_gains | k_gains) % 16:
         raise TensorError("rows and gains for an 8-bit cache begin at whole 16 bytes")
+    if write_kv and slots is None:
+        raise TensorError("keys and values to be written without their slots")
     places = _fits(slots, "slots", torch.int32, n, device) if write_kv else 0
     _check(library().pl_qk_norm_rope_kv_write_8bit(
         source, queries, stride, q_gains, k_gains, gain_code, float(eps), cosines, sines, rot, angles, 1 if neighbours else 0, _fits(positions, "positions", torch.int32, n, device), places,
@@ -3109,7 +3113,8 @@ def paged_attention_8bit(q: torch.Tensor, q_row_stride: int, out: torch.Tensor, 
     rows past ``max_q_len`` of a request may be left out.  The caller answers for the pages of all keys that are seen; what a row does not see
     may hold anything: a NaN there reaches the rows that see it and no other."""
     device = torch.cuda.current_device()
-    max_q_len, min_q_len, max_ctx, window = int(max_q_len), int(min_q_len), int(max_ctx), int(window or 0)
+    max_q_len, min_q_len, max_ctx = int(max_q_len), int(min_q_len), int(max_ctx)
+    window = min(max(int(window or 0), 1 - 2 ** 31), 2 ** 31 - 1)          # (no context is as long: more hides nothing either)
     code = _code(q, "query buffer")
     if nkv < 1 or nq < 1 or nq % nkv:
         raise TensorError(f"{nq} query heads over {nkv} key heads, which do not group evenly")
@@ -3120,10 +3125,10 @@ def paged_attention_8bit(q: torch.Tensor, q_row_stride: int, out: torch.Tensor, 
     S, width = block_table.shape if block_table.dim() == 2 else (0, 0)
     if S < 1 or width < 1:
         raise TensorError(f"block table has shape {tuple(block_table.shape)}, expected [requests, pages]")
-    if not 1 <= max_q_len <= n or not 0 <= min_q_len <= max_q_len or max_ctx < 1:
+    if not 1 <= max_q_len <= n or not 0 <= min_q_len <= max_q_len or not 1 <= max_ctx <= 2 ** 31 - 64:
         raise TensorError(f"requests are said to bring {min_q_len} to {max_q_len} of the step's {n} tokens, contexts to be {max_ctx} at most")
-    if not 0 < scale < math.inf:
-        raise TensorError(f"scores scaled by {scale}, which has to be finite and above zero")
+    if not 2.0 ** -126 <= scale <= 2.0 ** 126:
+        raise TensorError(f"scores scaled by {scale}, which has to be above zero and, times log2(e) too, a 32-bit number")
     queries, results = _fits(q, "query buffer", q.dtype, n * q_row_stride, device), _fits(out, "attention output", q.dtype, n * nq * d, device, (n, nq * d))
     if q_row_stride % 8 or (queries | results) % 16:
         raise TensorError("query rows and outputs for an 8-bit cache begin at whole 16 bytes")
