@@ -105,6 +105,8 @@ class Engine:
             raise ConfigError(f"sampler {sampler!r}, which is neither device nor host")
         if cache_dtype not in ("auto", "e4m3"):
             raise ConfigError(f"cache dtype {cache_dtype!r}, which is neither auto nor e4m3")
+        if cache_dtype == "e4m3" and kernels.attention() != "kernel":
+            raise ConfigError("cache dtype e4m3: the plain attention kernel (attention tensor) reads no pages held in 8 bits")
         self.dtype = dtype
         self.cache_dtype = dtype if cache_dtype == "auto" else cache_dtype
         self.model_dir = Path(model)

@@ -582,6 +582,11 @@ def set_attention(mode: str) -> None:
     _attention_mode = mode
 
 
+def attention() -> str:
+    """What ``set_attention`` has set."""
+    return _attention_mode
+
+
 # The figures of the estimate below: what a compute unit takes in from memory (bytes a microsecond); what a workgroup costs it
 # beside that; and what sharing costs the launch, where the shares meet in the kernel, where a second kernel puts them together, and
 # where that one has more than 16 of them, which it fetches in several trips (microseconds).
