@@ -104,3 +104,26 @@ def test_values_past_the_largest_bfloat16(dtype):
         late = c - q + torch.arange(q, device=cache.DEV) >= position
         assert not bool(rows[late][:, 1, :, [7, 9]].isfinite().any())
         assert bool(rows[~late].isfinite().all()) and bool(rows[late][:, 1, :, 10:].isfinite().all()) and bool(rows[late][:, 0].isfinite().all())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("requests,max_ctx", [([(150, 400), (5, 3000), (3, 900), (1, 50)], 3000), ([(2 + s % 4, 1500 + 97 * s) for s in range(40)], 60000), ([(700, 2500), (300, 300)], 2500)])
+def test_a_nan_value_among_shares(dtype, requests, max_ctx):
+    """Few rows beside many, whose shares stand in other places of the room; contexts that the kernel cuts itself; many rows in shares: NaN at the last tokens, before them, and far in front (which all rows see)."""
+    scene = cache.Scene(requests, 32, 8, 64, 16, dtype)
+    for window in (0, 70):
+        clean = scene.run(window, max_ctx=max_ctx)
+        scene.check(clean, window)
+        held = scene.pages.clone()
+        bad = torch.zeros(scene.n, 8, 4, 64, dtype=torch.bool, device=cache.DEV)
+        for s, (q, c) in enumerate(requests):
+            for position, head, columns in ((c - 1, 1, slice(None)), (c - 1 - q // 2, 2, slice(0, 5)), (max(c - q - 20, 0), 3, slice(7, 8)), (c // 5, 4, slice(None)), (c // 5, 5, slice(9, 10)), (c - 1, 5, slice(8, 12)),
+                                            (c - 1 - q // 3, 5, slice(40, 50))):
+                spoil(scene, s, position, head, columns)
+                bad[scene.starts[s]:scene.starts[s] + q, head, :, columns] |= seen_by(scene, s, window)[:, position].view(-1, 1, 1)
+        bad = bad.view(scene.n, -1)
+        out = scene.run(window, max_ctx=max_ctx)
+        assert bool(out[bad].isnan().all())
+        out[bad] = clean[bad]
+        scene.check(out, window)
+        scene.pages = held
