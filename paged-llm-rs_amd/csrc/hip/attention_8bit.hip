@@ -642,7 +642,7 @@ __global__ __launch_bounds__(A8_WAVES * PL_WAVE, (A8Few<PIECES, DQ>::WAVES(RB)))
             __syncthreads();
         }
         if (wave == 0 && out_row[b] >= 0) {
-            if (unlike) {
+            if (__builtin_expect(unlike, 0)) {
                 float finite = 0.f;              // (or NaN)
 #pragma unroll
                 for (int t = 0; t < 4 * DQ; ++t)
@@ -672,6 +672,7 @@ __global__ __launch_bounds__(A8_WAVES * PL_WAVE, (A8Few<PIECES, DQ>::WAVES(RB)))
             }
         }
     }
+    if (__builtin_expect(!unlike, 1)) return;
     again = static_cast<uint64_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(again >> 32))) << 32 | static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(again)));
     if (again == 0 || wave != 0 || (!BALANCED && whole_row && shares > 1)) return;
     __threadfence_block();
