@@ -13,7 +13,9 @@
 //                     are a reduction inside the lane and one exchange with lane ^ 32.
 //   O^T += V^T . P^T  the lane's weights are the B operand as they stand: V^T is read from LDS in the order in which the scores lie in the registers.
 //
-// Maximum, sum, weights and output are 32-bit; exponentials are base 2 with log2(e) folded into the scale.
+// Maximum, sum and output are 32-bit.  In bfloat16 the weights of the second product are rounded to bfloat16 (2^-8 at most each), as in the other attention kernels here, since that product would take twice as long with two
+// numbers a weight: outputs are 0.0018 of their size from 64 bits, 0.0022 in the kernel of many rows, whose largest weight may be anything up to 2^8 and is rounded too; their own rounding to bfloat16 alone is 0.0017.
+// In 32 bits weights lose nothing.  Exponentials are base 2 with log2(e) folded into the scale.
 #include "common.hpp"
 
 typedef __bf16 a8_bf16x2 __attribute__((ext_vector_type(2)));
@@ -691,8 +693,8 @@ __global__ __launch_bounds__(A8_WAVES * PL_WAVE, (A8Few<PIECES, DQ>::WAVES(RB)))
 // What bounds it is what a SIMD can issue: of a tile of 64 keys and 128 values a wave's products take 1,024 cycles, its other vector instructions some 1,060 (an exponential as long as two of the rest), and LDS,
 // which every wave reads whole, another 500 a wave and its share of the unit.  So the scores of the next tile are multiplied while the weights of this one are made, and the next maximum is found while
 // this tile's weights meet its values: both pipes work in one wave, whatever the other wave of the SIMD does.  For that the keys in LDS are a tile ahead of the values (two lengths of keys, three of
-// values), their bytes another tile ahead in registers, and their pages one more.  A round has one barrier.  8,100 tokens of 32 heads over 8 take 0.53 ms, 1,010 TFLOP/s (a large matrix product of the library
-// reaches 1,450 on the same card); without the overlap 0.69.  Tried and slower: the two waves of a SIMD half a round apart with a barrier a half (0.64), 64 rows a wave with all 512 registers (0.85: moves
+// values), their bytes another tile ahead in registers, and their pages one more.  A round has one barrier.  8,100 tokens of 32 heads over 8 take 0.515 ms, 1,045 TFLOP/s (0.50 to 0.56 as the card clocks;
+// a large matrix product of the library reaches 1,450 on the same card); without the overlap they took 0.69 when that was 0.57.  Tried and slower: the two waves of a SIMD half a round apart with a barrier a half (0.64), 64 rows a wave with all 512 registers (0.85: moves
 // between the two halves of the register file).
 template <int PIECES, int DT>
 struct A8Many {

@@ -139,7 +139,8 @@ extern "C" int pl_step_tables(const void* q_len, const void* ctx_len, int S, voi
 // Rows of heads are taken eight values a lane, d / 8 lanes a row.  A run is what the step brings to one page: rows that follow each other with slots that follow
 // each other.  One wave or workgroup takes a run of one key head, keys or values: the largest of its rows gives the page's new power, then the rows are
 // rounded into the page.  Runs of more rows than it takes at a time are read (and normed, turned) twice, the second time from L2.  Queries are normed and turned by workgroups of their own in the
-// same launch.  Prompts are bound by what they read and write (10,503 rows of 32 + 8 heads of 128: 237 MB in 77 us, 3.1 TB/s), single tokens by the waits for slots, rows and powers one behind the other (64 of 16 + 8 heads: 5.4 us).
+// same launch.  Prompts are bound by what they read and write (10,503 rows of 32 + 8 heads of 128: 237 MB in 70 us where inputs change from call to call, 3.4 TB/s; 60 us on the same ones), single tokens by the waits for slots, rows and powers one behind the other (64 of 16 + 8 heads: 5.4 us),
+// and steps in between by a wave's chain of these for every run, all its rows a few at a time and twice (788 rows in 32 bits into 4 heads of 64: 9.1 us, their bytes 1.5).
 struct P8Write {
     const void* qkv;
     void* q;
@@ -424,8 +425,8 @@ struct P8Shape {
 };
 static P8Shape p8_shape(int n, int nkv, int block, int d) {
     // A wave takes a run, 64 / LPR rows at a time; in steps of many rows a workgroup does, four times as many.  It looks through `tile` rows for the first ones of runs: one each while all of a
-    // step's may be first (decoding), else 32, since most of many rows are inside a page, and units that find nothing still cost their start: 10,503 rows of prompts into 8 heads take 182 us with a
-    // workgroup a row and 77 with 32 rows, 600 single tokens 30 us with a workgroup each and 14 with a wave.  (Values of more rows held in registers, so that a run is not read again from L2 once its
+    // step's may be first (decoding), else 32, since most of many rows are inside a page, and units that find nothing still cost their start: 10,503 rows of prompts into 8 heads took 182 us with a
+    // workgroup a row and 77 with 32 rows when this was chosen (70 now), 600 single tokens 30 us with a workgroup each and 14 with a wave.  (Values of more rows held in registers, so that a run is not read again from L2 once its
     // power is known, cost the queries' workgroups of the same launch their places: 94 us with twice the rows, 117 with four times.)
     const int tile = static_cast<long>(n) * 2 * nkv <= P8_SINGLE_UNITS ? 1 : 32;
     return P8Shape{tile, tile > 1 && block > PL_WAVE / p8_lanes(d) ? P8_WAVES : 1};

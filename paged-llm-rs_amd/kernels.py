@@ -3114,8 +3114,9 @@ def paged_attention_8bit(q: torch.Tensor, q_row_stride: int, out: torch.Tensor, 
     many of them, under ``window`` < 0 those of its own block of -window positions.  ``q`` rows begin with the rotated queries, ``q_row_stride`` apart.  Rows of no request, and of requests whose context is shorter than what they bring, are left
     as they were in ``out``.
 
-    ``max_q_len``, ``min_q_len`` and ``max_ctx`` bound what the requests bring and their contexts (the launches are sized and chosen by them): rows whose keys reach past ``max_ctx`` come out as NaN, and
-    rows past ``max_q_len`` of a request may be left out.  The caller answers for the pages of all keys that are seen; what a row does not see
+    ``max_q_len``, ``min_q_len`` (of those that bring any) and ``max_ctx`` bound what the requests bring and their contexts: the launches are sized and chosen by them.  Where a request brings more or fewer, rows of any
+    request may be left as they were.  Where a context is longer, its rows come out as NaN once the keys that they see are more than the launch has shares for (``shares_8bit``: max_ctx rounded up to whole
+    shares, or under a window what it reaches), and are what they should be until then.  The caller answers for the pages of all keys that are seen; what a row does not see
     may hold anything: a NaN there reaches the rows that see it and no other."""
     device = torch.cuda.current_device()
     max_q_len, min_q_len, max_ctx = int(max_q_len), int(min_q_len), int(max_ctx)
